@@ -20,6 +20,9 @@ SYMBOLS = [
     "cuhnsw_last_build_counters", "cuhnsw_debug_gather_probe", "cuhnsw_last_search_trails",
     "cuhnsw_last_search_side_by_side", "cuhnsw_literal_fallbacks", "cuhnsw_trails_available",
     "cuhnsw_num_deleted", "cuhnsw_search_knn_taking", "cuhnsw_last_search_team", "cuhnsw_last_build_team_batches",
+    "cuhnsw_get_items", "cuhnsw_search_items", "cuhnsw_get_labels", "cuhnsw_pack_items", "cuhnsw_lookup_rows",
+    "cuhnsw_lookup_grad_workspace", "cuhnsw_lookup_rows_grad", "cuhnsw_pack_rows", "cuhnsw_packed_scores_workspace",
+    "cuhnsw_packed_scores", "cuhnsw_select_beams_workspace", "cuhnsw_select_beams", "cuhnsw_reorder_states",
 ]
 
 _lib = None
@@ -67,6 +70,23 @@ def load():
   l.cuhnsw_trails_available.argtypes = [vp]
   l.cuhnsw_num_deleted.argtypes = [vp]
   l.cuhnsw_set_tunable.argtypes = [vp, ctypes.c_char_p, cd]
+  ll, cf = ctypes.c_longlong, ctypes.c_float
+  l.cuhnsw_get_items.argtypes = [vp, vp, ci, cf, vp]
+  l.cuhnsw_search_items.argtypes = [vp, vp, ci, cf, ci, ci, vp, vp, vp]
+  l.cuhnsw_get_labels.argtypes = [vp, vp]
+  l.cuhnsw_pack_items.argtypes = [vp, ci, vp, vp, vp, ci, vp]
+  l.cuhnsw_lookup_rows.argtypes = [vp, ci, ll, ll, ci, vp, ci, ll, cf, vp, ci, vp]
+  l.cuhnsw_lookup_grad_workspace.argtypes = [ll, ll, ci]
+  l.cuhnsw_lookup_grad_workspace.restype = ll
+  l.cuhnsw_lookup_rows_grad.argtypes = [vp, ci, ll, vp, ci, ll, ll, ci, cf, vp, ci, vp, ll, vp]
+  l.cuhnsw_pack_rows.argtypes = [vp, ci, ll, ll, ci, ci, vp, vp, vp, ci, vp]
+  l.cuhnsw_packed_scores_workspace.argtypes = [ll, ci, ci, ci, ci]
+  l.cuhnsw_packed_scores_workspace.restype = ll
+  l.cuhnsw_packed_scores.argtypes = [vp, vp, vp, ci, ll, ci, ci, vp, ci, ll, ci, cf, vp, vp, ci, ll, vp, ll, vp]
+  l.cuhnsw_select_beams_workspace.argtypes = [ci, ci, ci, ci]
+  l.cuhnsw_select_beams_workspace.restype = ll
+  l.cuhnsw_select_beams.argtypes = [vp, ci, ll, ll, ci, ci, ci, vp, vp, ci, ci, ci, vp, vp, vp, vp, ll, vp]
+  l.cuhnsw_reorder_states.argtypes = [vp, vp, vp, vp, vp, ci, vp, ll, ll, ci, ci, ci, vp]
   _lib = l
   return l
 

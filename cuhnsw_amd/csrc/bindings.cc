@@ -3,6 +3,7 @@
 // js1010/cuhnsw), implemented as a thin shim over the C ABI in include/cuhnsw_amd.h.
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
 
 #include <sched.h>
 
@@ -86,6 +87,50 @@ class CuHNSWBind {
   int MaxLevel() const { return cuhnsw_max_level(obj_); }
   int EnterPoint() const { return cuhnsw_enter_point(obj_); }
   double LastBuildSeconds() const { return cuhnsw_last_build_seconds(obj_); }
+  void GetItems(py::object& items, float scale, py::object& out) {
+    int_array _items(items);
+    float_array _out(out);
+    if (_items.ndim() != 1) throw std::runtime_error("items must be 1d array");
+    if ((long long)_out.size() < (long long)_items.size() * cuhnsw_num_dims(obj_)) throw std::runtime_error("output array is too small");
+    const int* in = _items.data();
+    float* to = _out.mutable_data();
+    const int num = (int)_items.size();
+    int rc;
+    {
+      py::gil_scoped_release release;
+      rc = cuhnsw_get_items(obj_, in, num, scale, to);
+    }
+    Check(rc);
+  }
+  void SearchItems(py::object& items, float scale, int topk, int ef_search, py::object& nns, py::object& distances, py::object& found_cnt) {
+    int_array _items(items);
+    int_array _nns(nns);
+    float_array _distances(distances);
+    int_array _found_cnt(found_cnt);
+    if (_items.ndim() != 1) throw std::runtime_error("items must be 1d array");
+    const long long num = (long long)_items.size();
+    if ((long long)_nns.size() < num * topk || (long long)_distances.size() < num * topk || (long long)_found_cnt.size() < num)
+      throw std::runtime_error("output arrays are too small");
+    const int* in = _items.data();
+    int* out_nns = _nns.mutable_data();
+    float* out_distances = _distances.mutable_data();
+    int* out_found = _found_cnt.mutable_data();
+    int rc;
+    {
+      py::gil_scoped_release release;
+      rc = cuhnsw_search_items(obj_, in, (int)num, scale, topk, ef_search, out_nns, out_distances, out_found);
+    }
+    Check(rc);
+  }
+  py::array_t<long long> GetLabels() {
+    py::array_t<long long> out(cuhnsw_num_data(obj_));
+    Check(cuhnsw_get_labels(obj_, out.mutable_data()));
+    return out;
+  }
+  void PackItems(int group, uintptr_t codes, uintptr_t scales, uintptr_t offsets, int scale_type, uintptr_t stream) {
+    Check(cuhnsw_pack_items(obj_, group, (void*)codes, (void*)scales, (void*)offsets, scale_type, (void*)stream));
+  }
+  int NumDeleted() const { return cuhnsw_num_deleted(obj_); }
   void SetTunable(std::string name, double value) {
     const int rc = cuhnsw_set_tunable(obj_, name.c_str(), value);
     if (rc == -2) throw std::runtime_error("tunable " + name + " has to be set before set_data / load_index");
@@ -124,7 +169,61 @@ static void CopyBytes(py::array dst, py::array src) {
   for (std::thread& t : threads) t.join();
 }
 
+// The operators on rows: addresses as integers, the message of the thread's last failed call as an exception.
+static void CheckCall(int rc) {
+  if (rc != 0) throw std::runtime_error(cuhnsw_last_error(nullptr));
+}
+static void LookupRows(uintptr_t table, int table_type, long long num_rows, long long row_stride, int num_dims, uintptr_t ids, int ids_64,
+                       long long num_ids, float scale, uintptr_t out, int out_type, uintptr_t stream) {
+  CheckCall(cuhnsw_lookup_rows((void*)table, table_type, num_rows, row_stride, num_dims, (void*)ids, ids_64, num_ids, scale, (void*)out,
+                               out_type, (void*)stream));
+}
+static void LookupRowsGrad(uintptr_t grad, int grad_type, long long grad_stride, uintptr_t ids, int ids_64, long long num_ids,
+                           long long num_rows, int num_dims, float scale, uintptr_t out, int out_type, uintptr_t workspace,
+                           long long workspace_bytes, uintptr_t stream) {
+  CheckCall(cuhnsw_lookup_rows_grad((void*)grad, grad_type, grad_stride, (void*)ids, ids_64, num_ids, num_rows, num_dims, scale, (void*)out,
+                                    out_type, (void*)workspace, workspace_bytes, (void*)stream));
+}
+static void PackRows(uintptr_t rows, int type, long long row_stride, long long num_rows, int num_dims, int group, uintptr_t codes,
+                     uintptr_t scales, uintptr_t offsets, int scale_type, uintptr_t stream) {
+  CheckCall(cuhnsw_pack_rows((void*)rows, type, row_stride, num_rows, num_dims, group, (void*)codes, (void*)scales, (void*)offsets, scale_type,
+                             (void*)stream));
+}
+static void PackedScores(uintptr_t codes, uintptr_t scales, uintptr_t offsets, int scale_type, long long num_rows, int num_dims, int group,
+                         uintptr_t queries, int query_type, long long query_stride, int num_queries, float alpha, uintptr_t bias,
+                         uintptr_t out, int out_type, long long out_stride, uintptr_t workspace, long long workspace_bytes, uintptr_t stream) {
+  CheckCall(cuhnsw_packed_scores((void*)codes, (void*)scales, (void*)offsets, scale_type, num_rows, num_dims, group, (void*)queries, query_type,
+                                 query_stride, num_queries, alpha, (const float*)bias, (void*)out, out_type, out_stride, (void*)workspace,
+                                 workspace_bytes, (void*)stream));
+}
+static void SelectBeams(uintptr_t scores, int type, long long stride_b, long long stride_k, int num_batch, int num_beams, int num_values,
+                        uintptr_t beams, uintptr_t finished, int end, int normalise, int num, uintptr_t totals, uintptr_t parents,
+                        uintptr_t tokens, uintptr_t workspace, long long workspace_bytes, uintptr_t stream) {
+  CheckCall(cuhnsw_select_beams((void*)scores, type, stride_b, stride_k, num_batch, num_beams, num_values, (const float*)beams,
+                                (const unsigned char*)finished, end, normalise, num, (float*)totals, (int*)parents, (int*)tokens,
+                                (void*)workspace, workspace_bytes, (void*)stream));
+}
+static void ReorderStates(const std::vector<uintptr_t>& from, const std::vector<uintptr_t>& to, const std::vector<long long>& stride_b,
+                          const std::vector<long long>& stride_k, const std::vector<long long>& bytes, uintptr_t parents,
+                          long long parent_stride_b, long long parent_stride_k, int num_batch, int num_beams, int num_picked,
+                          uintptr_t stream) {
+  const size_t n = from.size();
+  if (to.size() != n || stride_b.size() != n || stride_k.size() != n || bytes.size() != n) throw std::runtime_error("reorder: lists of one length are wanted");
+  CheckCall(cuhnsw_reorder_states(reinterpret_cast<const void* const*>(from.data()), reinterpret_cast<void* const*>(to.data()), stride_b.data(),
+                                  stride_k.data(), bytes.data(), (int)n, (const int*)parents, parent_stride_b, parent_stride_k, num_batch,
+                                  num_beams, num_picked, (void*)stream));
+}
+
 PYBIND11_MODULE(cuhnsw_bind, m) {
+  m.def("lookup_rows", &LookupRows);
+  m.def("lookup_rows_grad", &LookupRowsGrad);
+  m.def("lookup_grad_workspace", &cuhnsw_lookup_grad_workspace);
+  m.def("pack_rows", &PackRows);
+  m.def("packed_scores", &PackedScores);
+  m.def("packed_scores_workspace", &cuhnsw_packed_scores_workspace);
+  m.def("select_beams", &SelectBeams);
+  m.def("select_beams_workspace", &cuhnsw_select_beams_workspace);
+  m.def("reorder_states", &ReorderStates);
   m.def("copy_bytes", &CopyBytes, py::arg("dst"), py::arg("src"));
   m.def("has_device", []() { return cuhnsw_has_device() != 0; });
   py::class_<CuHNSWBind>(m, "CuHNSWBind")
@@ -137,6 +236,13 @@ PYBIND11_MODULE(cuhnsw_bind, m) {
       .def("load_index", &CuHNSWBind::LoadIndex, py::arg("fpath"))
       .def("search_knn", &CuHNSWBind::SearchGraph, py::arg("qdata"), py::arg("topk"), py::arg("ef_search"),
            py::arg("nns"), py::arg("distances"), py::arg("found"))
+      .def("get_items", &CuHNSWBind::GetItems, py::arg("items"), py::arg("scale"), py::arg("out"))
+      .def("search_items", &CuHNSWBind::SearchItems, py::arg("items"), py::arg("scale"), py::arg("topk"), py::arg("ef_search"),
+           py::arg("nns"), py::arg("distances"), py::arg("found"))
+      .def("get_labels", &CuHNSWBind::GetLabels)
+      .def("pack_items", &CuHNSWBind::PackItems, py::arg("group"), py::arg("codes"), py::arg("scales"), py::arg("offsets"),
+           py::arg("scale_type"), py::arg("stream"))
+      .def("num_deleted", &CuHNSWBind::NumDeleted)
       .def("num_data", &CuHNSWBind::NumData)
       .def("num_dims", &CuHNSWBind::NumDims)
       .def("max_level", &CuHNSWBind::MaxLevel)

@@ -1,5 +1,6 @@
 // C ABI of libcuhnsw_amd.so.
 #include "engine.h"
+#include "engine_items.h"
 
 #include "../../include/cuhnsw_amd.h"
 
@@ -31,11 +32,12 @@ using cuhnsw_amd::Engine;
 
 struct cuhnsw_engine {
   Engine impl;
+  cuhnsw_amd::Items items;
   std::mutex mutex;  // calls on one engine are serialised: they share its staging buffers, slot pool and streams
 };
 
 namespace {
-thread_local std::string g_create_error;
+thread_local std::string g_call_error;  // of the last call without an engine (cuhnsw_create, the operators on rows) that failed
 
 template <typename F>
 int locked(cuhnsw_engine* e, F&& f) {  // (the engine's lock is held)
@@ -59,6 +61,14 @@ int guarded(cuhnsw_engine* e, F&& f) {
 }
 }  // namespace
 
+void cuhnsw_amd::set_call_error(const char* message) noexcept {
+  try {
+    g_call_error = message;
+  } catch (...) {
+    g_call_error.clear();
+  }
+}
+
 extern "C" {
 
 int cuhnsw_create(cuhnsw_engine** out) {
@@ -67,13 +77,13 @@ int cuhnsw_create(cuhnsw_engine** out) {
     *out = new cuhnsw_engine();
     return 0;
   } catch (const std::exception& ex) {
-    g_create_error = ex.what();
+    g_call_error = ex.what();
     *out = nullptr;
     return -1;
   }
 }
 void cuhnsw_destroy(cuhnsw_engine* e) { delete e; }
-const char* cuhnsw_last_error(cuhnsw_engine* e) { return e ? e->impl.err.c_str() : g_create_error.c_str(); }
+const char* cuhnsw_last_error(cuhnsw_engine* e) { return e ? e->impl.err.c_str() : g_call_error.c_str(); }
 
 int cuhnsw_init(cuhnsw_engine* e, const char* opt_path) {
   if (!e) return -1;
@@ -81,11 +91,15 @@ int cuhnsw_init(cuhnsw_engine* e, const char* opt_path) {
   return e->impl.init(opt_path);
 }
 int cuhnsw_set_data(cuhnsw_engine* e, const float* data, int num_data, int num_dims) {
-  return guarded(e, [&](Engine& g) { g.set_data(data, num_data, num_dims); });
+  return guarded(e, [&](Engine& g) {
+    e->items.forget();
+    g.set_data(data, num_data, num_dims);
+  });
 }
 int cuhnsw_set_random_levels(cuhnsw_engine* e, const int* levels, int num_levels) {
   return guarded(e, [&](Engine& g) {
     if (!levels) throw std::runtime_error("set_random_levels: null levels");
+    e->items.forget();
     g.set_random_levels(levels, num_levels);
   });
 }
@@ -94,7 +108,10 @@ int cuhnsw_save_index(cuhnsw_engine* e, const char* fpath) {
   return guarded(e, [&](Engine& g) { g.save_index(fpath ? fpath : ""); });
 }
 int cuhnsw_load_index(cuhnsw_engine* e, const char* fpath) {
-  return guarded(e, [&](Engine& g) { g.load_index(fpath ? fpath : ""); });
+  return guarded(e, [&](Engine& g) {
+    e->items.forget();
+    g.load_index(fpath ? fpath : "");
+  });
 }
 int cuhnsw_search_knn(cuhnsw_engine* e, const float* qdata, int num_queries, int topk, int ef_search, int* nns,
                       float* distances, int* found_cnt) {
@@ -136,6 +153,19 @@ int cuhnsw_search_knn_device_noalloc(cuhnsw_engine* e, const float* d_qdata, int
   return guarded(e, [&](Engine& g) {
     g.search_device(d_qdata, num_queries, topk, ef_search, d_nns, d_distances, d_found_cnt, nullptr, kernel_ms, true);
   });
+}
+int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, float scale, float* out) {
+  return guarded(e, [&](Engine& g) { e->items.get(g, items, num_items, scale, out); });
+}
+int cuhnsw_search_items(cuhnsw_engine* e, const int* items, int num_items, float scale, int topk, int ef_search, int* nns,
+                        float* distances, int* found_cnt) {
+  return guarded(e, [&](Engine& g) { e->items.search(g, items, num_items, scale, topk, ef_search, nns, distances, found_cnt); });
+}
+int cuhnsw_get_labels(cuhnsw_engine* e, long long* out) {
+  return guarded(e, [&](Engine& g) { e->items.labels(g, out); });
+}
+int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, void* offsets, int scale_type, void* stream) {
+  return guarded(e, [&](Engine& g) { e->items.pack(g, group, codes, scales, offsets, scale_type, static_cast<hipStream_t>(stream)); });
 }
 int cuhnsw_debug_gather_probe(cuhnsw_engine* e, int waves_per_cu, int rows_in_flight, int dependent, double* rows,
                               float* ms) {

@@ -73,6 +73,15 @@ def _copy_of(data):
   return rows
 
 
+def _item_array(items):
+  items = np.asarray(items)
+  if items.ndim != 1 or (items.size and items.dtype.kind not in "iu"):
+    raise ValueError("items are a list of whole numbers")
+  if items.size and (items.min() < 0 or items.max() > np.iinfo(np.int32).max):
+    raise ValueError("item %d is outside the index" % (items.min() if items.min() < 0 else items.max()))
+  return np.ascontiguousarray(items, dtype=np.int32)
+
+
 class CuHNSW:
   """HNSW index built and searched on the GPU."""
 
@@ -118,3 +127,26 @@ class CuHNSW:
     out = (np.empty((rows, topk), np.int32), np.empty((rows, topk), np.float32), np.empty(rows, np.int32))
     self.obj.search_knn(queries, topk, max(topk, ef_search), *out)
     return out
+
+  # -- the index's vectors as a table (not in the reference) --------------------------------------
+  # Items are named as search_knn names them: by label on a loaded index, else by row number.
+  def get_items(self, items, scale=1.0):
+    """The items' vectors as the index holds them, times scale: float32 [len(items), dims]."""
+    items = _item_array(items)
+    out = np.empty((items.shape[0], self.obj.num_dims()), np.float32)
+    self.obj.get_items(items, scale, out)
+    return out
+
+  def search_items(self, items, topk, ef_search, scale=1.0):
+    """search_knn with the items' own vectors, times scale, as queries: they stay on the GPU."""
+    items = _item_array(items)
+    rows = items.shape[0]
+    out = (np.empty((rows, topk), np.int32), np.empty((rows, topk), np.float32), np.empty(rows, np.int32))
+    self.obj.search_items(items, scale, topk, max(topk, ef_search), *out)
+    return out
+
+  def pack_rows(self, group=32, offsets=None):
+    """All vectors in 4 bits (rows.PackedRows, in the current device's memory), for exact scores and searches over every
+    row.  Offsets suit vectors that are not centred; by default they go with dist_type l2.  Needs torch, imported first."""
+    from cuhnsw_amd import rows
+    return rows.pack_index(self, group, self.opt.dist_type == "l2" if offsets is None else offsets)

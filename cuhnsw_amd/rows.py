@@ -1,0 +1,384 @@
+"""Operators on tables of learned vectors that are on the GPU, as torch tensors: what a user of the index needs next to it.
+
+  lookup(table, ids, scale)        rows by id, differentiable: queries made of items, a model's input embedding
+  pack(vectors) -> PackedRows      rows in 4 bits with a scale per group of elements
+  PackedRows.scores(queries)       products with every row: the exact form of what a search answers approximately
+  PackedRows.search_knn(...)       the best rows of all, as CuHNSW.search_knn returns them
+  select_beams(scores, ...)        the best candidates over beams and vocabulary; over one beam: the nearest neighbours
+  reorder_states(states, parents)  the beams' states in their new order
+
+Every call runs on its tensors' device and torch's current stream there, does not wait for the GPU, takes its scratch
+memory from torch, and may be captured into a graph.  Wrong arguments are a ValueError (a TypeError where the kind of
+object is wrong); what the native library refuses is a RuntimeError with its message, as everywhere in this package.
+There is no CPU form.
+
+torch ships its own copy of the HIP runtime: it has to be imported before this package's native library is loaded, or
+the process holds two runtimes that do not know each other's memory.
+"""
+import sys
+
+if "torch" not in sys.modules and "cuhnsw_amd.cuhnsw_bind" in sys.modules:
+  raise ImportError("cuhnsw_amd.rows: import torch before cuhnsw_amd (two HIP runtimes would be loaded otherwise)")
+
+import numbers
+
+import numpy as np
+import torch
+
+try:
+  from cuhnsw_amd import cuhnsw_bind as _native
+except ImportError as exc:  # pragma: no cover
+  raise ImportError("cuhnsw_amd: the native extension is missing (%s); build it with `python -m cuhnsw_amd.build`" % exc) from exc
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_GROUPS = (32, 64, 128)
+
+
+def _check(ok, message, *args):
+  if not ok:
+    raise ValueError(message % args)
+
+
+def _tensor(x, name, dims=None, types=_TYPES):
+  if not isinstance(x, torch.Tensor):
+    raise TypeError("%s is a tensor, not %s" % (name, type(x).__name__))
+  _check(dims is None or x.dim() == dims, "%s has %s dimensions, %s are wanted", name, x.dim(), dims)
+  _check(x.dtype in types, "%s has the type %s: %s is wanted", name, x.dtype, " or ".join(str(t) for t in types))
+
+
+def _rows(x, name):
+  """The row stride of a matrix whose rows are contiguous, whatever lies between them (an expanded one's is 0)."""
+  _check(x.shape[1] <= 1 or x.stride(1) == 1, "the elements of one row of %s have to be contiguous", name)
+  return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _same_device(first, *others):
+  _check(first.is_cuda, "the tensors have to be on the GPU")
+  for x in others:
+    _check(x is None or x.device == first.device, "the tensors are on different devices")
+
+
+def _number(x, name):
+  if not isinstance(x, numbers.Real) or isinstance(x, bool):
+    raise TypeError("%s is a number, not %s" % (name, type(x).__name__))
+  return float(x)
+
+
+def _stream(device):
+  return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on(device):
+  return torch.cuda.device(device)
+
+
+def _workspace(size, device):
+  return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _address(x):
+  return 0 if x is None else x.data_ptr()
+
+
+# -------------------------------------------------------------------------------------------------- lookup
+_IDS = {torch.int32: 0, torch.int64: 1}
+
+
+def _lookup(table, ids, scale, dtype):
+  stride = _rows(table, "table")
+  flat = ids.reshape(-1)
+  out = torch.empty(flat.shape[0], table.shape[1], dtype=dtype, device=table.device)
+  if flat.stride(0) != 1:
+    flat = flat.contiguous()
+  with _on(table.device):
+    _native.lookup_rows(table.data_ptr(), _TYPES[table.dtype], table.shape[0], stride, table.shape[1], flat.data_ptr(), _IDS[ids.dtype],
+                        flat.shape[0], scale, out.data_ptr(), _TYPES[dtype], _stream(table.device))
+  return out.view(*ids.shape, table.shape[1])
+
+
+class _Lookup(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, table, ids, scale, dtype):
+    ctx.save_for_backward(ids)
+    ctx.scale, ctx.num_rows, ctx.dtype = scale, table.shape[0], table.dtype
+    return _lookup(table, ids, scale, dtype)
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, grad):
+    ids, = ctx.saved_tensors
+    return lookup_grad(grad, ids, ctx.num_rows, ctx.scale, ctx.dtype), None, None, None
+
+
+def lookup(table, ids, scale=1.0, dtype=None):
+  """scale * table[ids], zeros where an id is outside [0, len(table)) (padded places: -1).
+
+  table: [rows, dims], float32, float16 or bfloat16, rows contiguous; ids: int32 or int64 of any shape; the result, of
+  shape [*ids.shape, dims], has the table's type or is float32.  Products are taken in 32 bits and rounded once.
+  Differentiable with respect to table (once): see lookup_grad."""
+  _tensor(table, "table", 2)
+  _tensor(ids, "ids", types=_IDS)
+  scale = _number(scale, "scale")
+  dtype = dtype or table.dtype
+  _check(dtype in (table.dtype, torch.float32), "the result has the table's type or is float32")
+  _check(table.shape[1] > 0, "the table's rows are empty")
+  _same_device(table, ids)
+  if table.requires_grad and torch.is_grad_enabled():
+    return _Lookup.apply(table, ids, scale, dtype)
+  return _lookup(table, ids, scale, dtype)
+
+
+def lookup_grad(grad, ids, num_rows, scale=1.0, dtype=None):
+  """The gradient of lookup with respect to its table: [num_rows, dims], row v the sum of scale * grad[t] over the places
+  t with ids[t] = v.
+
+  grad: [*ids.shape, dims].  The sums run over the places in ascending order, in 32 bits, rounded once to `dtype`
+  (grad's own, or any where grad is float32): the same inputs give the same bits, whatever the device does meanwhile."""
+  _tensor(grad, "grad")
+  _tensor(ids, "ids", types=_IDS)
+  scale = _number(scale, "scale")
+  dtype = dtype or grad.dtype
+  _check(dtype in _TYPES and (grad.dtype in (dtype, torch.float32)), "the gradient of a %s table is of that type or float32", dtype)
+  _check(grad.dim() == ids.dim() + 1 and grad.shape[:-1] == ids.shape, "grad has the shape [*ids.shape, dims]")
+  _check(grad.shape[-1] > 0, "the rows of grad are empty")
+  _check(isinstance(num_rows, int) and num_rows >= 0, "num_rows is a whole number that is not negative")
+  _same_device(grad, ids)
+  dims, flat = grad.shape[-1], ids.reshape(-1).contiguous()
+  grad = grad.reshape(-1, dims)
+  if dims > 1 and grad.stride(1) != 1:
+    grad = grad.contiguous()
+  out = torch.empty(num_rows, dims, dtype=dtype, device=grad.device)
+  with _on(grad.device):
+    size = _native.lookup_grad_workspace(flat.shape[0], num_rows, dims)
+    work = _workspace(size, grad.device)
+    _native.lookup_rows_grad(grad.data_ptr(), _TYPES[grad.dtype], _rows(grad, "grad"), flat.data_ptr(), _IDS[ids.dtype], flat.shape[0],
+                             num_rows, dims, scale, out.data_ptr(), _TYPES[dtype], _address(work), size, _stream(grad.device))
+  return out
+
+
+# -------------------------------------------------------------------------------------------- rows in 4 bits
+_SCALES = {torch.float16: 1, torch.bfloat16: 2}
+
+
+class PackedRows:
+  """Rows held in 4 bits: element k of row n is scales[n][k // group] * (code - 8) or, with offsets,
+  scales[n][k // group] * code + offsets[n][k // group].
+
+  codes: uint8 [rows, 16 * ceil(num_dims / 32)], element 2 i in the low half of byte i (what is behind num_dims elements is
+  not looked at); scales, offsets: float16 or bfloat16 [rows, ceil(num_dims / group)]; group: 32, 64 or 128.  The tensors are
+  used as they are, not copied.  labels: int64 [rows], what search_knn returns instead of row numbers, or None."""
+
+  def __init__(self, codes, scales, offsets=None, *, num_dims, group=32, labels=None):
+    _check(isinstance(num_dims, int) and num_dims > 0, "num_dims is a positive whole number")
+    _check(group in _GROUPS, "the group is 32, 64 or 128 elements")
+    _tensor(codes, "codes", 2, (torch.uint8,))
+    _tensor(scales, "scales", 2, _SCALES)
+    width, groups = 16 * -(-num_dims // 32), -(-num_dims // group)
+    _check(codes.shape[1] == width, "codes of %d elements are %d bytes a row", num_dims, width)
+    _check(tuple(scales.shape) == (codes.shape[0], groups), "scales have the shape (%d, %d)", codes.shape[0], groups)
+    if offsets is not None:
+      _tensor(offsets, "offsets", 2, (scales.dtype,))
+      _check(offsets.shape == scales.shape, "offsets have the shape of scales")
+    if labels is not None:
+      _tensor(labels, "labels", 1, (torch.int64,))
+      _check(labels.shape[0] == codes.shape[0], "there is one label a row")
+    for name, x in (("codes", codes), ("scales", scales), ("offsets", offsets)):
+      _check(x is None or x.is_contiguous(), "%s have to be contiguous", name)
+    _check(codes.data_ptr() % 16 == 0, "codes have to be aligned to 16 bytes")
+    _same_device(codes, scales, offsets, labels)
+    self.codes, self.scales, self.offsets, self.labels = codes, scales, offsets, labels
+    self.num_rows, self.num_dims, self.group = codes.shape[0], num_dims, group
+    self._norms = None
+
+  def __len__(self):
+    return self.num_rows
+
+  def scores(self, queries, alpha=1.0, bias=None, dtype=None):
+    """alpha * queries @ rows.T (+ bias): [num_queries, num_rows], of the queries' type or float32.
+
+    queries: [num_queries, num_dims] (or one: [num_dims]), float32, float16 or bfloat16; bias: float32 [num_rows].  Sums are
+    held in 32 bits.  A query that is not finite gets scores that are not."""
+    _tensor(queries, "queries")
+    _check(queries.dim() in (1, 2) and queries.shape[-1] == self.num_dims, "queries have the shape [num_queries, %d]", self.num_dims)
+    alpha = _number(alpha, "alpha")
+    dtype = dtype or queries.dtype
+    _check(dtype in (queries.dtype, torch.float32), "the scores have the queries' type or are float32")
+    if bias is not None:
+      _tensor(bias, "bias", 1, (torch.float32,))
+      _check(bias.shape[0] == self.num_rows and bias.is_contiguous(), "bias is contiguous, one value a row")
+    _same_device(self.codes, queries, bias)
+    q = queries if queries.dim() == 2 else queries[None]
+    stride = _rows(q, "queries")
+    nq, device = q.shape[0], q.device
+    out = torch.empty(nq, self.num_rows, dtype=dtype, device=device)
+    with _on(device):
+      kind = _TYPES[q.dtype]
+      size = _native.packed_scores_workspace(self.num_rows, self.num_dims, self.group, kind, nq)
+      work = _workspace(size, device)
+      _native.packed_scores(self.codes.data_ptr(), self.scales.data_ptr(), _address(self.offsets), _SCALES[self.scales.dtype], self.num_rows,
+                            self.num_dims, self.group, q.data_ptr(), kind, stride, nq, alpha, _address(bias), out.data_ptr(),
+                            _TYPES[dtype], self.num_rows, _address(work), size, _stream(device))
+    return out if queries.dim() == 2 else out[0]
+
+  def unpack(self):
+    """The rows as float32 [num_rows, num_dims]."""
+    values = torch.stack((self.codes & 15, self.codes >> 4), dim=2).view(self.num_rows, -1)[:, :self.num_dims].float()
+    column = torch.arange(self.num_dims, device=self.codes.device) // self.group
+    scales = self.scales.float()[:, column]
+    return (values - 8.0) * scales if self.offsets is None else values * scales + self.offsets.float()[:, column]
+
+  def norms(self):
+    """Squared lengths of the rows, float32 (computed once: the rows must not change afterwards)."""
+    if self._norms is None:
+      out = torch.empty(self.num_rows, dtype=torch.float32, device=self.codes.device)
+      step = max(1, (64 << 20) // self.num_dims)
+      for low in range(0, self.num_rows, step):
+        part = PackedRows(self.codes[low:low + step], self.scales[low:low + step],
+                          None if self.offsets is None else self.offsets[low:low + step], num_dims=self.num_dims, group=self.group)
+        out[low:low + step] = part.unpack().double().square_().sum(1)
+      self._norms = out
+    return self._norms
+
+  def search_knn(self, queries, topk, dist_type="dot"):
+    """The topk (up to 256) nearest of all rows: (ids int32, or int64 labels, distances float32, found int32), nearest first and of
+    equal ones the lower row first, as CuHNSW.search_knn's: -<q, row> for "dot", squared distances for "l2"."""
+    _check(dist_type in ("dot", "l2"), "dist_type is dot or l2, not %s", dist_type)
+    _tensor(queries, "queries")
+    q = queries if queries.dim() == 2 else queries[None]
+    _check(q.dim() == 2 and q.shape[1] == self.num_dims, "queries have the shape [num_queries, %d]", self.num_dims)
+    _check(isinstance(topk, int) and 0 < topk <= 256, "topk is between 1 and 256")
+    _same_device(self.codes, q)
+    l2 = dist_type == "l2"
+    bias = -self.norms() if l2 else None
+    lengths = q.double().square().sum(1, keepdim=True) if l2 else None
+    step = max(1, (1 << 30) // max(1, self.num_rows))  # (scores of at most 4 GiB at a time)
+    found = []
+    for low in range(0, max(1, q.shape[0]), step):
+      part = self.scores(q[low:low + step], alpha=2.0 if l2 else 1.0, bias=bias, dtype=torch.float32)
+      found.append(select_beams(part[:, None, :], None, topk, normalise=False))
+    best, _, ids = (torch.cat(x) for x in zip(*found)) if len(found) > 1 else found[0]
+    there = ids >= 0
+    distances = (lengths - best.double()).clamp_min(0.0).float() if l2 else -best
+    distances = torch.where(there, distances, float("inf"))
+    if self.labels is not None:
+      ids = torch.where(there, self.labels[ids.clamp_min(0).long()], -1)
+    return ids, distances, there.sum(1, dtype=torch.int32)
+
+
+def _empty_packed(num_rows, num_dims, group, offsets, scale_dtype, device):
+  _check(group in _GROUPS, "the group is 32, 64 or 128 elements")
+  _check(scale_dtype in _SCALES, "scales are float16 or bfloat16")
+  groups = -(-num_dims // group)
+  codes = torch.empty(num_rows, 16 * -(-num_dims // 32), dtype=torch.uint8, device=device)
+  scales = torch.empty(num_rows, groups, dtype=scale_dtype, device=device)
+  return codes, scales, torch.empty_like(scales) if offsets else None
+
+
+def pack(vectors, group=32, offsets=False, scale_dtype=torch.float16, labels=None):
+  """The nearest PackedRows of finite vectors [rows, dims] (float32, float16 or bfloat16): per group scale = largest magnitude
+  / 7, or with offsets (for vectors that are not centred) scale = span / 15 and offset = the smallest."""
+  _tensor(vectors, "vectors", 2)
+  _check(vectors.shape[1] > 0, "the vectors are empty")
+  stride = _rows(vectors, "vectors")
+  _check(group in _GROUPS, "the group is 32, 64 or 128 elements")
+  _check(scale_dtype in _SCALES, "scales are float16 or bfloat16")
+  _same_device(vectors)
+  n, d = vectors.shape
+  codes, scales, lows = _empty_packed(n, d, group, offsets, scale_dtype, vectors.device)
+  with _on(vectors.device):
+    _native.pack_rows(vectors.data_ptr(), _TYPES[vectors.dtype], stride, n, d, group, codes.data_ptr(), scales.data_ptr(), _address(lows),
+                      _SCALES[scale_dtype], _stream(vectors.device))
+  return PackedRows(codes, scales, lows, num_dims=d, group=group, labels=labels)
+
+
+def pack_index(index, group=32, offsets=False, scale_dtype=torch.float16):
+  """PackedRows of the vectors that a CuHNSW index holds (CuHNSW.pack_rows).  Rows of a loaded index keep its labels; an index
+  with deleted elements is refused, since its rows are all returned here."""
+  obj = index.obj
+  if obj.num_deleted() > 0:
+    raise RuntimeError("pack_rows: the index holds deleted elements")
+  _check(obj.num_data() > 0, "pack_rows: no vectors (call set_data or load_index first)")
+  _check(torch.cuda.is_available(), "no HIP device available: this call needs a GPU")
+  device = torch.device("cuda", torch.cuda.current_device())
+  n, d = obj.num_data(), obj.num_dims()
+  codes, scales, lows = _empty_packed(n, d, group, offsets, scale_dtype, device)
+  obj.pack_items(group, codes.data_ptr(), scales.data_ptr(), _address(lows), _SCALES[scale_dtype], _stream(device))
+  labels = obj.get_labels()
+  plain = np.array_equal(labels, np.arange(n))
+  return PackedRows(codes, scales, lows, num_dims=d, group=group, labels=None if plain else torch.from_numpy(labels).to(device))
+
+
+# ------------------------------------------------------------------------------------------------- selection
+def select_beams(scores, beams, num, normalise=True, finished=None, end=None):
+  """The `num` (1 to 256) best candidates of every batch entry over its beams and the vocabulary: (totals float32, parents
+  int32, tokens int32), each [batch, num], best first.
+
+  scores: [batch, beams, values], float32, float16 or bfloat16; beams: float32 [batch, beams], what the beams have gathered, or
+  None (zeros).  A candidate's total is beams + scores, with normalise beams + log_softmax(scores); totals are compared in 64
+  bits, equal ones go to the lower beam, then the larger score, then the lower token.  Masked places hold -infinity (a NaN counts as
+  one): they are never chosen, and where too few candidates are left the rest says -infinity, -1, -1.  finished: bool
+  [batch, beams] or None: a finished beam has one candidate, token `end`, with what it gathered."""
+  _tensor(scores, "scores", 3)
+  _check(isinstance(num, int) and 0 < num <= 256, "num is between 1 and 256")
+  b, k, v = scores.shape
+  _check(k > 0 and v > 0, "there are no beams or no values")
+  _check(k * min(num, v) <= 4096, "%d beams and %d candidates: at most 4096 together", k, num)
+  _check(v == 1 or scores.stride(2) == 1, "the values of one beam have to be contiguous")
+  if beams is not None:
+    _tensor(beams, "beams", 2, (torch.float32,))
+    _check(tuple(beams.shape) == (b, k), "beams have the shape (%d, %d)", b, k)
+  if finished is not None:
+    _tensor(finished, "finished", 2, (torch.bool,))
+    _check(tuple(finished.shape) == (b, k), "finished has the shape (%d, %d)", b, k)
+    _check(beams is not None, "finished beams need what they gathered (beams)")
+    _check(isinstance(end, int) and 0 <= end < v, "finished beams need the token that ends a sequence (end)")
+  _same_device(scores, beams, finished)
+  device = scores.device
+  beams = None if beams is None else beams.contiguous()
+  finished = None if finished is None else finished.contiguous()
+  totals = torch.empty(b, num, dtype=torch.float32, device=device)
+  parents = torch.empty(b, num, dtype=torch.int32, device=device)
+  tokens = torch.empty(b, num, dtype=torch.int32, device=device)
+  with _on(device):
+    size = _native.select_beams_workspace(b, k, v, num)
+    work = _workspace(size, device)
+    _native.select_beams(scores.data_ptr(), _TYPES[scores.dtype], scores.stride(0), scores.stride(1), b, k, v, _address(beams),
+                         _address(finished), 0 if end is None else end, int(bool(normalise)), num, totals.data_ptr(), parents.data_ptr(),
+                         tokens.data_ptr(), _address(work), size, _stream(device))
+  return totals, parents, tokens
+
+
+def reorder_states(states, parents):
+  """What the beams remember, in their new order: for every tensor [batch, beams, ...] of states a new one [batch, picked, ...]
+  whose entry [b][j] is the old one's [b][parents[b][j]], zeros where that is outside [0, beams).
+
+  states: a list of tensors of any type, one beam's state contiguous; parents: int32 [batch, picked] (select_beams')."""
+  _tensor(parents, "parents", 2, (torch.int32,))
+  if isinstance(states, torch.Tensor):
+    raise TypeError("states is a list of tensors")
+  states = list(states)
+  if not states:
+    return []
+  b, picked = parents.shape
+  first = states[0]
+  outs, sizes = [], []
+  for x in states:
+    if not isinstance(x, torch.Tensor):
+      raise TypeError("states is a list of tensors")
+    _check(x.dim() >= 2 and x.shape[0] == b and x.shape[1] == first.shape[1] and x.shape[1] > 0,
+           "states have the shape [batch, beams, ...]: %s with %d batch entries", tuple(x.shape), b)
+    expected = 1
+    for size, stride in zip(reversed(x.shape[2:]), reversed(x.stride()[2:])):
+      _check(size == 1 or stride == expected, "one beam's state has to be contiguous")
+      expected *= size
+    sizes.append(expected * x.element_size())
+  _check(b * picked <= 65535, "at most 65535 states in all")
+  _same_device(parents, *states)
+  for x in states:
+    outs.append(torch.empty(b, picked, *x.shape[2:], dtype=x.dtype, device=x.device))
+  with _on(parents.device):
+    _native.reorder_states([x.data_ptr() for x in states], [x.data_ptr() for x in outs], [x.stride(0) * x.element_size() for x in states],
+                           [x.stride(1) * x.element_size() for x in states], sizes, parents.data_ptr(), parents.stride(0), parents.stride(1),
+                           b, first.shape[1], picked, _stream(parents.device))
+  return outs

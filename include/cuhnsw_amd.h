@@ -269,6 +269,79 @@ int cuhnsw_trails_available(cuhnsw_engine* e);
  * returns -1 for an unknown name */
 int cuhnsw_set_tunable(cuhnsw_engine* e, const char* name, double value);
 
+/* ---- the index's vectors as a table ---------------------------------------------------------------
+ * Items are named as a search names them: by label on an index that came from a file, else by row number.
+ *
+ * cuhnsw_get_items: out[i][:] = scale * vector of items[i], float32 [num_items, num_dims] (with fp16_storage the
+ *   rounded vector).  Host pointers.  An item that is not in the index is an error.
+ * cuhnsw_search_items: cuhnsw_search_knn with these vectors as queries; they never leave the GPU.
+ * cuhnsw_get_labels: the label of every row (its number where the index did not come from a file).
+ * cuhnsw_pack_items: all vectors in 4 bits (cuhnsw_pack_rows) into device memory of the caller's, on the caller's
+ *   stream (NULL = the default stream); has ended when the call returns. */
+int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, float scale, float* out);
+int cuhnsw_search_items(cuhnsw_engine* e, const int* items, int num_items, float scale, int topk, int ef_search, int* nns,
+                        float* distances, int* found_cnt);
+int cuhnsw_get_labels(cuhnsw_engine* e, long long* out);
+int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, void* offsets, int scale_type, void* stream);
+
+/* ---- operators on tables of vectors ----------------------------------------------------------------
+ * No engine: device pointers of the current HIP device and a hipStream_t (NULL = the default stream).  Unlike the calls
+ * above these only launch: they return before the GPU is done, allocate nothing and wait for nothing, and may be recorded
+ * into a HIP graph.  `workspace` is scratch memory of the caller's, of at least as many bytes as the call named ..._workspace
+ * says (0 for bad sizes); nothing is kept in it between calls, but two launches that may run at once need one each.
+ * Returns 0, or -1 with the message in cuhnsw_last_error(NULL) (per thread).
+ * Element types: 0 = float32, 1 = float16, 2 = bfloat16.  Strides are in elements, and the elements of one row are
+ * contiguous.  Sums are held in 32 bits or more and rounded once.
+ *
+ * cuhnsw_lookup_rows: out[t] = scale * table[ids[t]], zeros where ids[t] is outside [0, num_rows) (padded places: -1).
+ *   ids: int32, or int64 with ids_64; out: dense [num_ids, num_dims], of the table's type or float32.
+ * cuhnsw_lookup_rows_grad: out[v] = scale * sum of grad[t] over the t with ids[t] = v, t ascending: the result does not
+ *   depend on how the work was spread.  All of out is written: dense [num_rows, num_dims], of the gradient's type, or
+ *   of any where that is float32.  num_ids <= 2^30, num_rows < 2^31 - 1. */
+int cuhnsw_lookup_rows(const void* table, int table_type, long long num_rows, long long row_stride, int num_dims, const void* ids,
+                       int ids_64, long long num_ids, float scale, void* out, int out_type, void* stream);
+long long cuhnsw_lookup_grad_workspace(long long num_ids, long long num_rows, int num_dims);
+int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stride, const void* ids, int ids_64, long long num_ids,
+                            long long num_rows, int num_dims, float scale, void* out, int out_type, void* workspace,
+                            long long workspace_bytes, void* stream);
+
+/* Rows in 4 bits.  A row's codes (0 to 15) take 16 bytes for every 32 elements, element 2 i in the low half of byte i;
+ * every `group` (32, 64 or 128) elements have a scale and perhaps an offset, of scale_type 1 or 2:
+ *   element = scale * (code - 8), or scale * code + offset.
+ * codes: [num_rows, 16 * ceil(num_dims / 32)] aligned to 16 bytes; scales, offsets: [num_rows, ceil(num_dims / group)].
+ *
+ * cuhnsw_pack_rows: the nearest such rows of finite ones (scale = largest magnitude / 7, or the span / 15 with offsets).
+ * cuhnsw_packed_scores: out[m][n] = alpha * <row n, query m> + bias[n] (bias: float32 [num_rows] or NULL), of the queries'
+ *   type or float32.  A query that holds an infinity or a NaN gets NaN or infinities; other queries are not touched by it. */
+int cuhnsw_pack_rows(const void* rows, int type, long long row_stride, long long num_rows, int num_dims, int group, void* codes,
+                     void* scales, void* offsets, int scale_type, void* stream);
+long long cuhnsw_packed_scores_workspace(long long num_rows, int num_dims, int group, int query_type, int num_queries);
+int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offsets, int scale_type, long long num_rows, int num_dims,
+                         int group, const void* queries, int query_type, long long query_stride, int num_queries, float alpha,
+                         const float* bias, void* out, int out_type, long long out_stride, void* workspace, long long workspace_bytes,
+                         void* stream);
+
+/* Selection over the beams of a search and a vocabulary.
+ * cuhnsw_select_beams: of every batch entry b the `num` (1 to 256) largest of
+ *     beams[b][k] + scores[b][k][v]                       or, with normalise,
+ *     beams[b][k] + scores[b][k][v] - log(sum over u of exp(scores[b][k][u]))
+ *   over k and v, largest first; of equal totals (held in 64 bits) the lower k first, then the larger score, then the lower
+ *   v.  beams: float32 [num_batch, num_beams] or NULL (zeros).  A NaN counts as -infinity and -infinity is never chosen: places
+ *   that are left over say -infinity, -1, -1.  finished (bytes, [num_batch, num_beams]) or NULL: where it is not 0 the beam
+ *   has one candidate, token `end` with total beams[b][k].  num_beams * min(num, num_values) <= 4096.  Results: dense
+ *   [num_batch, num].  (One beam, not normalised: the num nearest neighbours of a matrix of scores.)
+ * cuhnsw_reorder_states: for each of num_states arrays to[b][j] = from[b][parents[b][j]], zeros where the parent is outside
+ *   [0, num_beams).  Host arrays of device pointers, of byte strides between batch entries and beams, and of the bytes of one
+ *   beam's state (contiguous); the results are dense [num_batch, num_picked, bytes] and must not overlap their sources.
+ *   Strides of parents in elements. */
+long long cuhnsw_select_beams_workspace(int num_batch, int num_beams, int num_values, int num);
+int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long long stride_k, int num_batch, int num_beams, int num_values,
+                        const float* beams, const unsigned char* finished, int end, int normalise, int num, float* out_totals,
+                        int* out_parents, int* out_tokens, void* workspace, long long workspace_bytes, void* stream);
+int cuhnsw_reorder_states(const void* const* from, void* const* to, const long long* stride_b, const long long* stride_k,
+                          const long long* bytes, int num_states, const int* parents, long long parent_stride_b,
+                          long long parent_stride_k, int num_batch, int num_beams, int num_picked, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
