@@ -15,22 +15,27 @@
 
 namespace cuhnsw_amd {
 
-constexpr int kMostNum = 256, kMostLists = 4096;
+constexpr int kMostNum = 256, kMostBeams = 1024, kMostLists = 4096;
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kKept = 2048;  // candidates a workgroup holds in LDS
 
 struct SelectArgs {
   const void* scores;
   long long stride_b, stride_k;
   int num_batch, num_beams, num_values;
-  const float* beams;            // [num_batch, num_beams] or null
+  const float* beams;             // [num_batch, num_beams] or null
   const unsigned char* finished;  // the same, or null
   int normalise, end, num;
   float* out_totals;
   int *out_parents, *out_tokens;
-  double* list_totals;  // per beam: its best min(num, num_values), largest first
-  int* list_tokens;
+  int parts, each;     // workgroups of a row, tiles of each of them
+  int most;            // min(num, num_values)
+  uint64_t* lists;     // per row and part: its `most` best, largest first; 0 where there are not so many
+  float* list_top;     // per row and part: the largest score,
+  double* list_sum;    // and the sum of exp(score - largest)
 };
 
-// Orders as the values do, +0 and -0 as one; larger keys first means lower places first among equals.
+// Orders as the values do, +0 and -0 as one; larger keys first means lower places first among equals.  No key is 0.
 __device__ inline uint64_t order_key(float x, uint32_t place) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~place;
@@ -39,93 +44,339 @@ __device__ inline float key_value(uint64_t key) {
   const uint32_t u = (uint32_t)(key >> 32);
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
+__device__ inline int key_place(uint64_t key) { return (int)~(uint32_t)key; }
 __device__ inline float score_at(float x) { return fmaxf(x, -INFINITY); }  // (of a NaN: the other operand)
 
+// the lanes' values, largest in lane 0
 template <typename T>
-__global__ void __launch_bounds__(256) select_row_kernel(SelectArgs a) {
-  __shared__ uint64_t best[256];
-  __shared__ double sums[256];
-  const int row = blockIdx.x, b = row / a.num_beams, k = row - b * a.num_beams, tid = threadIdx.x;
-  const T* x = static_cast<const T*>(a.scores) + b * a.stride_b + k * a.stride_k;
-  const int m = min(a.num, a.num_values);
-  const float beam = a.beams ? a.beams[row] : 0.f;
-  double* totals = a.list_totals + (long long)row * m;
-  int* tokens = a.list_tokens + (long long)row * m;
-  if (a.finished && a.finished[row]) {
-    for (int i = tid; i < m; i += 256) {
-      totals[i] = i == 0 ? (double)beam : -INFINITY;
-      tokens[i] = a.end;
+__device__ inline T sorted_lanes(T x) {
+  const int lane = threadIdx.x & 63;
+  for (int size = 2; size <= 64; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      const T other = __shfl_xor(x, step);
+      const bool larger_first = (lane & size) == 0 || size == 64, low = (lane & step) == 0;
+      x = (low == larger_first) == (other > x) ? other : x;
     }
-    return;
-  }
-  uint64_t under = ~0ull;
-  double top = 0.0, log_sum = 0.0;
-  for (int i = 0; i < m; ++i) {
-    uint64_t mine = 0;
-    for (int v = tid; v < a.num_values; v += 256) {
-      const uint64_t key = order_key(score_at(widen(x[v])), (uint32_t)v);
-      if (key < under && key > mine) mine = key;
-    }
-    best[tid] = mine;
-    __syncthreads();
-    for (int step = 128; step > 0; step >>= 1) {
-      if (tid < step && best[tid + step] > best[tid]) best[tid] = best[tid + step];
-      __syncthreads();
-    }
-    under = best[0];
-    __syncthreads();
-    const float value = key_value(under);
-    if (i == 0 && a.normalise) {
-      top = value;
-      double sum = 0.0;
-      for (int v = tid; v < a.num_values; v += 256) {
-        const float y = score_at(widen(x[v]));
-        sum += y == value ? 1.0 : (double)expf(y - value);
+  return x;
+}
+
+// A value that at least `num` of the workgroup's threads' `mine` are not below: of every wavefront the value that
+// ceil(num / 4) of its lanes reach, the smallest of the four.
+template <typename T>
+__device__ inline T reached_by(T mine, int num, T* shared) {
+  const T sorted = sorted_lanes(mine);
+  const int r = (num + kWaves - 1) / kWaves;
+  if ((threadIdx.x & 63) == r - 1) shared[threadIdx.x >> 6] = sorted;
+  __syncthreads();
+  T least = shared[0];
+  for (int w = 1; w < kWaves; ++w) least = shared[w] < least ? shared[w] : least;
+  return least;
+}
+
+// The best of `count` different keys to the front, in order; how many there are then (at most `most`).  Up to two for every thread are
+// ranked by counting the larger ones, more go through a bitonic network.
+__device__ inline int keep_best(uint64_t* keys, int count, int most) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (count <= 2 * kThreads) {
+    uint64_t mine[2];
+    int rank[2] = {0, 0};
+    for (int j = 0; j < 2; ++j) mine[j] = tid + j * kThreads < count ? keys[tid + j * kThreads] : 0;
+    if (count <= kThreads)
+      for (int i = 0; i < count; ++i) rank[0] += keys[i] > mine[0];
+    else
+      for (int i = 0; i < count; ++i) {
+        const uint64_t other = keys[i];
+        rank[0] += other > mine[0];
+        rank[1] += other > mine[1];
       }
-      sums[tid] = sum;
+    __syncthreads();
+    for (int j = 0; j < 2; ++j)
+      if (mine[j] && rank[j] < most) keys[rank[j]] = mine[j];
+  } else {
+    int size = 1024;
+    while (size < count) size <<= 1;
+    for (int i = count + tid; i < size; i += kThreads) keys[i] = 0;
+    for (int run = 2; run <= size; run <<= 1)
+      for (int step = run >> 1; step > 0; step >>= 1) {
+        __syncthreads();
+        for (int i = tid; i < size / 2; i += kThreads) {
+          const int a = (i / step) * 2 * step + i % step, b = a + step;
+          const uint64_t x = keys[a], y = keys[b];
+          if ((x < y) == ((a & run) == 0)) {
+            keys[a] = y;
+            keys[b] = x;
+          }
+        }
+      }
+  }
+  __syncthreads();
+  return min(count, most);
+}
+
+// Pass over a row's scores: each thread has EACH of a tile in registers.  The first tile gives a value that `num` of its scores
+// reach; what is not below it goes to a list in LDS.  A list that would overflow is cut down to its best, and what is left
+// to enter then has to beat the worst of them.
+template <typename T, int EACH>
+__global__ void __launch_bounds__(kThreads) select_part_kernel(SelectArgs a) {
+  constexpr int VE = 16 / sizeof(T), NV = EACH / VE;
+  __shared__ uint64_t kept[kKept];
+  __shared__ float shared[kWaves];
+  __shared__ double shared_sum[kWaves];
+  __shared__ int filled;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, b = row / a.num_beams, k = row - b * a.num_beams;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (a.finished && a.finished[row]) return;
+  const T* x = static_cast<const T*>(a.scores) + b * a.stride_b + k * a.stride_k;
+  const int ahead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));  // places of the first vector before the row
+  if (tid == 0) filled = 0;
+  __syncthreads();
+  int have = 0;
+  uint64_t bar_key = 0;   // what a key has to be above, once the list was cut
+  float bar = -INFINITY;  // what a score has to reach
+  float top = -INFINITY, sum = 0.f;
+  const long long tile_size = (long long)kThreads * EACH;
+  for (int t = 0; t < a.each; ++t) {
+    const long long first = ((long long)part * a.each + t) * tile_size - ahead;
+    if (first >= a.num_values) break;
+    float v[EACH];
+    const bool inside = first >= 0 && first + tile_size <= a.num_values;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const long long at = first + ((long long)i * kThreads + tid) * VE;
+      if (inside || (at >= 0 && at + VE <= a.num_values)) {
+        const Pack<T, VE> p = *reinterpret_cast<const Pack<T, VE>*>(x + at);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) v[i * VE + j] = score_at(widen(p.at[j]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) v[i * VE + j] = at + j >= 0 && at + j < a.num_values ? score_at(widen(x[at + j])) : -INFINITY;
+      }
+    }
+    float largest = v[0];
+#pragma unroll
+    for (int i = 1; i < EACH; ++i) largest = fmaxf(largest, v[i]);
+    if (a.normalise) {
+      constexpr float kLog2e = 1.44269504f;
+      if (largest > top) {
+        sum *= __builtin_amdgcn_exp2f((top - largest) * kLog2e);
+        top = largest;
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      const float before = sum;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);
+      if (top == INFINITY) {  // (beside an infinite one only the infinite ones count)
+        sum = before;
+        for (int i = 0; i < EACH; ++i) sum += v[i] == INFINITY ? 1.f : 0.f;
+      }
+    }
+    if (t == 0) bar = reached_by(largest, a.most, shared);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mine += __popcll(__ballot(v[i] >= bar && v[i] > -INFINITY));
+    int at = 0;
+    if (lane == 0 && mine) at = atomicAdd(&filled, mine);
+    at = __shfl(at, 0);
+    __syncthreads();
+    const int now = filled;
+    auto place = [&](int i) { return (uint32_t)(first + ((long long)(i / VE) * kThreads + tid) * VE + i % VE); };
+    if (now <= kKept) {
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const bool in = v[i] >= bar && v[i] > -INFINITY;
+          const unsigned long long with = __ballot(in);
+          if (in) kept[at + __popcll(with & ((1ull << lane) - 1))] = order_key(v[i], place(i));
+          at += __popcll(with);
+        }
+      }
+      have = now;
       __syncthreads();
-      for (int step = 128; step > 0; step >>= 1) {
-        if (tid < step) sums[tid] += sums[tid + step];
+    } else {
+      for (int i = 0; i < EACH; ++i) {
+        if (i == 0 || have + kThreads > kKept) {
+          have = keep_best(kept, have, a.most);
+          if (have == a.most) {
+            bar_key = kept[have - 1];
+            bar = key_value(bar_key);
+          }
+          if (tid == 0) filled = have;
+          __syncthreads();
+        }
+        float value = v[0];
+#pragma unroll
+        for (int j = 1; j < EACH; ++j) value = i == j ? v[j] : value;
+        const uint64_t key = order_key(value, place(i));
+        if (value > -INFINITY && key > bar_key) kept[atomicAdd(&filled, 1)] = key;
+        __syncthreads();
+        have = filled;
         __syncthreads();
       }
-      log_sum = log(sums[0]);
     }
+  }
+  have = keep_best(kept, have, a.most);
+  uint64_t* list = a.lists + (long long)blockIdx.x * a.most;
+  for (int i = tid; i < a.most; i += kThreads) list[i] = i < have ? kept[i] : 0;
+  if (a.normalise) {
+    float most = top;
+    for (int step = 32; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
+    if (lane == 0) shared[wave] = most;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, shared[w]);
+    double part_sum = top == most ? (double)sum : sum * exp((double)top - (double)most);
+    if (top == -INFINITY) part_sum = 0.0;
+    for (int step = 32; step > 0; step >>= 1) part_sum += __shfl_xor(part_sum, step);
+    if (lane == 0) shared_sum[wave] = part_sum;
+    __syncthreads();
     if (tid == 0) {
-      double total = value;
-      if (a.normalise) total = (value == (float)top ? 0.0 : (double)value - top) - log_sum;
-      totals[i] = value == -INFINITY ? -INFINITY : (double)beam + total;
-      tokens[i] = (int)~(uint32_t)under;
+      for (int w = 1; w < kWaves; ++w) part_sum += shared_sum[w];
+      a.list_top[blockIdx.x] = most;
+      a.list_sum[blockIdx.x] = part_sum;
     }
   }
 }
 
-__global__ void __launch_bounds__(64) select_merge_kernel(SelectArgs a) {
-  const int b = blockIdx.x, lane = threadIdx.x, m = min(a.num, a.num_values), all = a.num_beams * m;
-  const double* totals = a.list_totals + (long long)b * all;
-  const int* tokens = a.list_tokens + (long long)b * all;
-  double last = INFINITY;
-  int last_at = -1;
+// Orders as the values do; 0 is below all of them.
+__device__ inline uint64_t order_total(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  return u & 0x8000000000000000ull ? ~u : u | 0x8000000000000000ull;
+}
+__device__ inline double total_value(uint64_t u) {
+  return __longlong_as_double((long long)(u & 0x8000000000000000ull ? u & 0x7fffffffffffffffull : ~u));
+}
+
+// The lists of a batch entry's beams and parts become its answer: the totals in 64 bits, those that num of the threads' best
+// reach in LDS, each ranked among them by (total, lower beam, its own order).
+__global__ void __launch_bounds__(kThreads) select_merge_kernel(SelectArgs a) {
+  __shared__ uint64_t kept_total[kKept], kept_key[kKept];
+  __shared__ int kept_beam[kKept];
+  __shared__ uint64_t shared[kWaves];
+  __shared__ int filled, first_best;
+  extern __shared__ double beam_less[];  // per beam: the logarithm of its sum, and its largest score behind
+  double* beam_top = beam_less + a.num_beams;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int per_beam = a.parts * a.most, all = a.num_beams * per_beam;
+  for (int k = tid; k < a.num_beams; k += kThreads) {
+    const long long row = (long long)b * a.num_beams + k;
+    double top = -INFINITY, sum = 0.0;
+    if (a.normalise && !(a.finished && a.finished[row])) {
+      for (int p = 0; p < a.parts; ++p) top = fmax(top, (double)a.list_top[row * a.parts + p]);
+      for (int p = 0; p < a.parts; ++p) {
+        const double t = a.list_top[row * a.parts + p], s = a.list_sum[row * a.parts + p];
+        if (t > -INFINITY) sum += t == top ? s : s * exp(t - top);
+      }
+    }
+    beam_top[k] = top;
+    beam_less[k] = a.normalise ? log(sum) : 0.0;
+  }
+  if (tid == 0) filled = 0;
+  __syncthreads();
+  auto key_of = [&](int c) { return a.lists[(long long)b * all + c]; };
+  auto total_of = [&](int c, uint64_t key) -> uint64_t {  // 0: no candidate
+    const int k = c / per_beam;
+    const long long row = (long long)b * a.num_beams + k;
+    const double beam = a.beams ? a.beams[row] : 0.f;
+    double total;
+    if (a.finished && a.finished[row]) {
+      if (c != k * per_beam) return 0;
+      total = beam;
+    } else {
+      if (key == 0) return 0;
+      total = key_value(key);
+      if (a.normalise) total = (total == beam_top[k] ? 0.0 : total - beam_top[k]) - beam_less[k];
+      total += beam;
+    }
+    return total > -INFINITY ? order_total(total) : 0;
+  };
+  uint64_t best = 0;
+  for (int c = tid; c < all; c += kThreads) {
+    const uint64_t t = total_of(c, key_of(c));
+    best = t > best ? t : best;
+  }
+  const uint64_t bar = reached_by(best, a.num, shared);
+  for (int c = tid; c < all; c += kThreads) {
+    const uint64_t key = key_of(c), t = total_of(c, key);
+    if (t == 0 || t < bar) continue;
+    const int at = atomicAdd(&filled, 1);
+    if (at >= kKept) continue;
+    const int k = c / per_beam;
+    kept_total[at] = t;
+    kept_key[at] = a.finished && a.finished[(long long)b * a.num_beams + k] ? (uint64_t)(uint32_t)~(uint32_t)a.end : key;
+    kept_beam[at] = k;
+  }
+  __syncthreads();
+  const int count = filled;
+  const long long out = (long long)b * a.num;
+  if (count <= kKept) {
+    for (int i = tid; i < count; i += kThreads) {
+      const uint64_t t = kept_total[i], key = kept_key[i];
+      const int k = kept_beam[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) {
+        const uint64_t other = kept_total[j];
+        if (other == t) rank += kept_beam[j] < k || (kept_beam[j] == k && kept_key[j] > key);
+        else rank += other > t;
+      }
+      if (rank < a.num) {
+        a.out_totals[out + rank] = (float)total_value(t);
+        a.out_parents[out + rank] = k;
+        a.out_tokens[out + rank] = key_place(key);
+      }
+    }
+    for (int i = count + tid; i < a.num; i += kThreads) {
+      a.out_totals[out + i] = -INFINITY;
+      a.out_parents[out + i] = a.out_tokens[out + i] = -1;
+    }
+    return;
+  }
+  // More equal totals than are held: one after the other, each the best of those behind the last one.
+  uint64_t last = ~0ull, last_key = 0;
+  int last_beam = -1;
   for (int i = 0; i < a.num; ++i) {
-    double best = -INFINITY;
-    int at = all;
-    for (int c = lane; c < all; c += 64) {
-      const double t = totals[c];
-      const bool left = t < last || (t == last && c > last_at);
-      if (left && t > best) best = t, at = c;
+    uint64_t mine = 0, mine_key = 0;
+    int mine_beam = 0;
+    auto before = [](uint64_t t, int k, uint64_t key, uint64_t t2, int k2, uint64_t key2) {
+      return t != t2 ? t > t2 : k != k2 ? k < k2 : key > key2;
+    };
+    for (int c = tid; c < all; c += kThreads) {
+      const int k = c / per_beam;
+      uint64_t key = key_of(c);
+      const uint64_t t = total_of(c, key);
+      if (t == 0) continue;
+      if (a.finished && a.finished[(long long)b * a.num_beams + k]) key = (uint64_t)(uint32_t)~(uint32_t)a.end;
+      if (last_beam >= 0 && !before(last, last_beam, last_key, t, k, key)) continue;
+      if (mine == 0 || before(t, k, key, mine, mine_beam, mine_key)) mine = t, mine_key = key, mine_beam = k;
     }
     for (int step = 1; step < 64; step <<= 1) {
-      const double t = __shfl_xor(best, step);
-      const int c = __shfl_xor(at, step);
-      if (t > best || (t == best && c < at)) best = t, at = c;
+      const uint64_t t = __shfl_xor(mine, step), key = __shfl_xor(mine_key, step);
+      const int k = __shfl_xor(mine_beam, step);
+      if (t != 0 && (mine == 0 || before(t, k, key, mine, mine_beam, mine_key))) mine = t, mine_key = key, mine_beam = k;
     }
-    const bool there = best > -INFINITY;
-    if (lane == 0) {
-      a.out_totals[(long long)b * a.num + i] = (float)best;
-      a.out_parents[(long long)b * a.num + i] = there ? at / m : -1;
-      a.out_tokens[(long long)b * a.num + i] = there ? tokens[at] : -1;
+    __syncthreads();
+    if (lane == 0) kept_total[tid >> 6] = mine, kept_key[tid >> 6] = mine_key, kept_beam[tid >> 6] = mine_beam;
+    __syncthreads();
+    if (tid == 0) {
+      int w = 0;
+      for (int o = 1; o < kWaves; ++o)
+        if (kept_total[o] != 0 && (kept_total[w] == 0 || before(kept_total[o], kept_beam[o], kept_key[o], kept_total[w], kept_beam[w], kept_key[w]))) w = o;
+      first_best = w;
+      const bool there = kept_total[w] != 0;
+      a.out_totals[out + i] = there ? (float)total_value(kept_total[w]) : -INFINITY;
+      a.out_parents[out + i] = there ? kept_beam[w] : -1;
+      a.out_tokens[out + i] = there ? key_place(kept_key[w]) : -1;
     }
-    last = best;
-    last_at = at;
+    __syncthreads();
+    last = kept_total[first_best];
+    last_key = kept_key[first_best];
+    last_beam = kept_beam[first_best];
+    if (last == 0) {  // (nothing is left)
+      for (int j = i + 1 + tid; j < a.num; j += kThreads) {
+        a.out_totals[out + j] = -INFINITY;
+        a.out_parents[out + j] = a.out_tokens[out + j] = -1;
+      }
+      return;
+    }
   }
 }
 
@@ -135,10 +386,29 @@ struct ReorderArgs {
   const unsigned char* from[kMostStates];
   unsigned char* to[kMostStates];
   long long stride_b[kMostStates], stride_k[kMostStates], bytes[kMostStates];  // in bytes; the results are dense
+  unsigned char width[kMostStates];  // bytes that move together: the widest that sizes, strides and addresses allow
   const int* parents;
   long long parent_stride_b, parent_stride_k;
   int num_beams, num_picked;
 };
+
+template <typename T>
+__device__ inline void copy_or_clear(const unsigned char* from, unsigned char* to, long long bytes, bool there) {
+  constexpr int kAtOnce = 4;
+  const long long n = bytes / (long long)sizeof(T), stride = (long long)gridDim.x * 256;
+  const T* in = reinterpret_cast<const T*>(from);
+  T* out = reinterpret_cast<T*>(to);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += kAtOnce * stride) {
+    T x[kAtOnce] = {};
+    if (there)
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (i + j * stride < n) x[j] = in[i + j * stride];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i + j * stride < n) out[i + j * stride] = x[j];
+  }
+}
 
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   const int s = blockIdx.z, row = blockIdx.y, b = row / a.num_picked, j = row - b * a.num_picked;
@@ -146,17 +416,43 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   const bool there = parent >= 0 && parent < a.num_beams;
   const unsigned char* from = a.from[s] + b * a.stride_b[s] + (there ? parent : 0) * a.stride_k[s];
   unsigned char* to = a.to[s] + row * a.bytes[s];
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.bytes[s]; i += (long long)gridDim.x * 256) to[i] = there ? from[i] : 0;
+  switch (a.width[s]) {
+    case 16: copy_or_clear<uint4>(from, to, a.bytes[s], there); break;
+    case 8: copy_or_clear<uint2>(from, to, a.bytes[s], there); break;
+    case 4: copy_or_clear<uint32_t>(from, to, a.bytes[s], there); break;
+    case 2: copy_or_clear<uint16_t>(from, to, a.bytes[s], there); break;
+    default: copy_or_clear<uint8_t>(from, to, a.bytes[s], there); break;
+  }
+}
+
+// How a selection is spread: tiles of 8 or 32 scores for each thread, and so many workgroups a row.
+struct SelectPlan {
+  bool small;
+  int parts, each;
+};
+static SelectPlan select_plan(int num_batch, int num_beams, int num_values, int num) {
+  SelectPlan p;
+  const long long rows = (long long)num_batch * num_beams;
+  const int most = std::min(num, num_values);
+  p.small = rows * num_values < 512ll * 8192;
+  const long long tile = kThreads * (p.small ? 8 : 32);
+  const int tiles = (int)((15 + tile - 1 + num_values) / tile);  // (a row may begin inside a vector)
+  const long long wanted = std::min<long long>({(2048 + rows - 1) / rows, 256, std::max<long long>(1, 16384 / ((long long)num_beams * most))});
+  p.each = (int)((tiles + wanted - 1) / wanted);
+  p.parts = (tiles + p.each - 1) / p.each;
+  return p;
 }
 
 struct SelectScratch {
-  double* totals;
-  int* tokens;
+  uint64_t* lists;
+  double* sums;
+  float* tops;
   size_t bytes;
-  SelectScratch(void* memory, long long rows, int num) {
+  SelectScratch(void* memory, long long rows, int parts, int most) {
     WorkspaceParts s(memory);
-    totals = s.part<double>((size_t)rows * num);
-    tokens = s.part<int>((size_t)rows * num);
+    lists = s.part<uint64_t>((size_t)rows * parts * most);
+    sums = s.part<double>((size_t)rows * parts);
+    tops = s.part<float>((size_t)rows * parts);
     bytes = s.used();
   }
 };
@@ -169,7 +465,8 @@ extern "C" {
 
 long long cuhnsw_select_beams_workspace(int num_batch, int num_beams, int num_values, int num) {
   if (num_batch <= 0 || num_beams <= 0 || num_values <= 0 || num <= 0) return 0;
-  return (long long)SelectScratch(nullptr, (long long)num_batch * num_beams, std::min(num, num_values)).bytes;
+  return (long long)SelectScratch(nullptr, (long long)num_batch * num_beams, select_plan(num_batch, num_beams, num_values, num).parts,
+                                  std::min(num, num_values)).bytes;
 }
 
 int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long long stride_k, int num_batch, int num_beams, int num_values,
@@ -180,20 +477,26 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
     want(num_batch >= 0 && num_beams > 0 && num_values > 0, "select: bad sizes");
     want(num > 0 && num <= kMostNum, "select: between 1 and 256 candidates can be asked for");
     want((long long)num_beams * std::min(num, num_values) <= kMostLists, "select: more than 4096 candidates of all beams (beams times candidates asked for)");
+    want(num_beams <= kMostBeams, "select: more than 1024 beams");
     want((long long)num_batch * num_beams <= 0x7fffffff, "select: too many rows");
     if (num_batch == 0) return;
     want(scores && out_totals && out_parents && out_tokens, "select: null argument");
     want(!finished || (end >= 0 && end < num_values), "select: the token that ends a sequence is outside the vocabulary");
-    const SelectScratch w(workspace, (long long)num_batch * num_beams, std::min(num, num_values));
+    const SelectPlan p = select_plan(num_batch, num_beams, num_values, num);
+    const long long rows = (long long)num_batch * num_beams;
+    const SelectScratch w(workspace, rows, p.parts, std::min(num, num_values));
     want(workspace && workspace_bytes >= (long long)w.bytes, "select: the workspace is too small");
+    want(rows * p.parts <= 0x7fffffff, "select: too many rows");
     const SelectArgs a{scores, stride_b, stride_k, num_batch, num_beams, num_values, beams, finished, normalise, end, num,
-                       out_totals, out_parents, out_tokens, w.totals, w.tokens};
+                       out_totals, out_parents, out_tokens, p.parts, p.each, std::min(num, num_values), w.lists, w.tops, w.sums};
     hipStream_t s = static_cast<hipStream_t>(stream);
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL(select_row_kernel<T>, dim3((unsigned)(num_batch * num_beams)), dim3(256), 0, s, a);
+      const dim3 grid((unsigned)(rows * p.parts));
+      if (p.small) hipLaunchKernelGGL((select_part_kernel<T, 8>), grid, dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((select_part_kernel<T, 32>), grid, dim3(kThreads), 0, s, a);
     });
-    hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)num_batch), dim3(64), 0, s, a);
+    hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)num_batch), dim3(kThreads), (size_t)num_beams * 16, s, a);
     HIP_CHECK(hipGetLastError());
   });
 }
@@ -217,7 +520,10 @@ int cuhnsw_reorder_states(const void* const* from, void* const* to, const long l
         a.stride_k[i] = stride_k[first + i];
         a.bytes[i] = bytes[first + i];
         want(a.bytes[i] >= 0 && (a.bytes[i] == 0 || (a.from[i] && a.to[i])), "reorder: null argument");
-        most = std::max(most, a.bytes[i]);
+        const uint64_t all = (uint64_t)a.bytes[i] | (uint64_t)a.stride_b[i] | (uint64_t)a.stride_k[i] | reinterpret_cast<uintptr_t>(a.from[i]) |
+                             reinterpret_cast<uintptr_t>(a.to[i]) | 16;
+        a.width[i] = (unsigned char)(all & (~all + 1));
+        most = std::max(most, a.bytes[i] / a.width[i]);
       }
       if (most == 0) continue;
       a.parents = parents;
@@ -225,7 +531,7 @@ int cuhnsw_reorder_states(const void* const* from, void* const* to, const long l
       a.parent_stride_k = parent_stride_k;
       a.num_beams = num_beams;
       a.num_picked = num_picked;
-      hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)std::min<long long>((most + 255) / 256, 1024), (unsigned)(num_batch * num_picked), (unsigned)count),
+      hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)std::min<long long>((most + 1023) / 1024, 256), (unsigned)(num_batch * num_picked), (unsigned)count),
                          dim3(256), 0, static_cast<hipStream_t>(stream), a);
       HIP_CHECK(hipGetLastError());
     }

@@ -323,6 +323,7 @@ def select_beams(scores, beams, num, normalise=True, finished=None, end=None):
   _check(isinstance(num, int) and 0 < num <= 256, "num is between 1 and 256")
   b, k, v = scores.shape
   _check(k > 0 and v > 0, "there are no beams or no values")
+  _check(k <= 1024, "%d beams: at most 1024", k)
   _check(k * min(num, v) <= 4096, "%d beams and %d candidates: at most 4096 together", k, num)
   _check(v == 1 or scores.stride(2) == 1, "the values of one beam have to be contiguous")
   if beams is not None:

@@ -328,7 +328,7 @@ int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offs
  *   over k and v, largest first; of equal totals (held in 64 bits) the lower k first, then the larger score, then the lower
  *   v.  beams: float32 [num_batch, num_beams] or NULL (zeros).  A NaN counts as -infinity and -infinity is never chosen: places
  *   that are left over say -infinity, -1, -1.  finished (bytes, [num_batch, num_beams]) or NULL: where it is not 0 the beam
- *   has one candidate, token `end` with total beams[b][k].  num_beams * min(num, num_values) <= 4096.  Results: dense
+ *   has one candidate, token `end` with total beams[b][k].  num_beams <= 1024, num_beams * min(num, num_values) <= 4096.  Results: dense
  *   [num_batch, num].  (One beam, not normalised: the num nearest neighbours of a matrix of scores.)
  * cuhnsw_reorder_states: for each of num_states arrays to[b][j] = from[b][parents[b][j]], zeros where the parent is outside
  *   [0, num_beams).  Host arrays of device pointers, of byte strides between batch entries and beams, and of the bytes of one

@@ -91,6 +91,9 @@ def test_infinite_scores():
   x[1, 1, [3, 400]] = INF
   _check(x, _beams(2, 2), 4)
   _check(x, _beams(2, 2), 4, normalise=False)
+  many = _scores(1, 1, 70_000, torch.float32)
+  many[0, 0, ::5000] = INF             # (in several stretches of the row)
+  _check(many, _beams(1, 1), 20)
   lowest = torch.full((1, 2, 500), torch.finfo(torch.float32).min, device="cuda")    # a mask of the type's lowest value
   lowest[0, 1, 44] = 0.0
   _check(lowest, _beams(1, 2), 6)
