@@ -83,7 +83,7 @@ def load():
   l.cuhnsw_packed_scores_workspace.argtypes = [ll, ci, ci, ci, ci]
   l.cuhnsw_packed_scores_workspace.restype = ll
   l.cuhnsw_packed_scores.argtypes = [vp, vp, vp, ci, ll, ci, ci, vp, ci, ll, ci, cf, vp, vp, ci, ll, vp, ll, vp]
-  l.cuhnsw_select_beams_workspace.argtypes = [ci, ci, ci, ci]
+  l.cuhnsw_select_beams_workspace.argtypes = [ci, ci, ci, ci, ci]
   l.cuhnsw_select_beams_workspace.restype = ll
   l.cuhnsw_select_beams.argtypes = [vp, ci, ll, ll, ci, ci, ci, vp, vp, ci, ci, ci, vp, vp, vp, vp, ll, vp]
   l.cuhnsw_reorder_states.argtypes = [vp, vp, vp, vp, vp, ci, vp, ll, ll, ci, ci, ci, vp]

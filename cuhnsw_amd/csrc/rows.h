@@ -45,6 +45,12 @@ struct alignas(sizeof(T) * N) Pack {
   T at[N];
 };
 
+// the same at any address that fits the elements
+template <typename T, int N>
+struct LoosePack {
+  T at[N];
+};
+
 // the message of the last call without an engine that failed in this thread (engine.hip)
 void set_call_error(const char* message) noexcept;
 

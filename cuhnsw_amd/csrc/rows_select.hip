@@ -47,29 +47,24 @@ __device__ inline float key_value(uint64_t key) {
 __device__ inline int key_place(uint64_t key) { return (int)~(uint32_t)key; }
 __device__ inline float score_at(float x) { return fmaxf(x, -INFINITY); }  // (of a NaN: the other operand)
 
-// the lanes' values, largest in lane 0
+// The num-th largest of the workgroup's threads' values, by counting: of the values that fewer than num are above, the
+// smallest.  `all` has a place for every thread.
 template <typename T>
-__device__ inline T sorted_lanes(T x) {
-  const int lane = threadIdx.x & 63;
-  for (int size = 2; size <= 64; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      const T other = __shfl_xor(x, step);
-      const bool larger_first = (lane & size) == 0 || size == 64, low = (lane & step) == 0;
-      x = (low == larger_first) == (other > x) ? other : x;
-    }
-  return x;
-}
-
-// A value that at least `num` of the workgroup's threads' `mine` are not below: of every wavefront the value that
-// ceil(num / 4) of its lanes reach, the smallest of the four.
-template <typename T>
-__device__ inline T reached_by(T mine, int num, T* shared) {
-  const T sorted = sorted_lanes(mine);
-  const int r = (num + kWaves - 1) / kWaves;
-  if ((threadIdx.x & 63) == r - 1) shared[threadIdx.x >> 6] = sorted;
+__device__ inline T reached_by(T mine, int num, T largest_possible, T* all) {
+  all[threadIdx.x] = mine;
   __syncthreads();
-  T least = shared[0];
-  for (int w = 1; w < kWaves; ++w) least = shared[w] < least ? shared[w] : least;
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < kThreads; ++i) above += all[i] > mine;
+  T least = above < num ? mine : largest_possible;
+  for (int step = 32; step > 0; step >>= 1) {
+    const T other = __shfl_xor(least, step);
+    least = other < least ? other : least;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) all[threadIdx.x >> 6] = least;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) least = all[w] < least ? all[w] : least;
   return least;
 }
 
@@ -82,14 +77,17 @@ __device__ inline int keep_best(uint64_t* keys, int count, int most) {
     uint64_t mine[2];
     int rank[2] = {0, 0};
     for (int j = 0; j < 2; ++j) mine[j] = tid + j * kThreads < count ? keys[tid + j * kThreads] : 0;
-    if (count <= kThreads)
+    if (count <= kThreads) {
+#pragma unroll 8
       for (int i = 0; i < count; ++i) rank[0] += keys[i] > mine[0];
-    else
+    } else {
+#pragma unroll 8
       for (int i = 0; i < count; ++i) {
         const uint64_t other = keys[i];
         rank[0] += other > mine[0];
         rank[1] += other > mine[1];
       }
+    }
     __syncthreads();
     for (int j = 0; j < 2; ++j)
       if (mine[j] && rank[j] < most) keys[rank[j]] = mine[j];
@@ -114,48 +112,61 @@ __device__ inline int keep_best(uint64_t* keys, int count, int most) {
   return min(count, most);
 }
 
-// Pass over a row's scores: each thread has EACH of a tile in registers.  The first tile gives a value that `num` of its scores
-// reach; what is not below it goes to a list in LDS.  A list that would overflow is cut down to its best, and what is left
-// to enter then has to beat the worst of them.
-template <typename T, int EACH>
-__global__ void __launch_bounds__(kThreads) select_part_kernel(SelectArgs a) {
-  constexpr int VE = 16 / sizeof(T), NV = EACH / VE;
+// Pass over a row's scores: NV vectors of 16 bytes for each thread are a tile, and the next tile is asked for before the one
+// at hand is looked at.  The first tile gives a value that `num` of its scores reach; what is not below it goes to a list in LDS,
+// which is cut down to its best after that tile and whenever it has grown long: what comes later has to reach the worst of
+// them.  Where a tile would overflow the list (scores in an order that is hard) it enters a score of each thread at a time.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) {
+  constexpr int VE = 16 / sizeof(T), EACH = NV * VE;
+  typedef LoosePack<T, VE> Vector;
   __shared__ uint64_t kept[kKept];
-  __shared__ float shared[kWaves];
+  __shared__ float shared[kThreads];
   __shared__ double shared_sum[kWaves];
   __shared__ int filled;
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, b = row / a.num_beams, k = row - b * a.num_beams;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (a.finished && a.finished[row]) return;
   const T* x = static_cast<const T*>(a.scores) + b * a.stride_b + k * a.stride_k;
-  const int ahead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));  // places of the first vector before the row
+  // Whole vectors of the row, wherever it begins (global memory takes 16 bytes from any address), and the scores behind them,
+  // which the first workgroup of the row takes one by one.  Which thread gets which score depends on the sizes alone: equal
+  // rows have the same sum to the last bit, and equal candidates of theirs are equal.
+  const int vectors = a.num_values / VE, tail = a.num_values - vectors * VE;
   if (tid == 0) filled = 0;
   __syncthreads();
+  constexpr int kTile = kThreads * NV;  // vectors
+  auto load = [&](int first, Vector (&to)[NV]) {
+    const T* from = x + (first + tid) * VE;
+    if (first + kTile <= vectors) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) to[i] = *reinterpret_cast<const Vector*>(from + i * (kThreads * VE));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) to[i].at[j] = narrow<T>(-INFINITY);
+        if (first + i * kThreads + tid < vectors) to[i] = *reinterpret_cast<const Vector*>(from + i * (kThreads * VE));
+      }
+    }
+  };
   int have = 0;
   uint64_t bar_key = 0;   // what a key has to be above, once the list was cut
   float bar = -INFINITY;  // what a score has to reach
   float top = -INFINITY, sum = 0.f;
-  const long long tile_size = (long long)kThreads * EACH;
-  for (int t = 0; t < a.each; ++t) {
-    const long long first = ((long long)part * a.each + t) * tile_size - ahead;
-    if (first >= a.num_values) break;
+  int first = part * a.each * kTile;
+  const int tiles = max(part == 0 ? 1 : 0, first < vectors ? min(a.each, (vectors - first + kTile - 1) / kTile) : 0);
+  const int extra_place = vectors * VE + tid;
+  float extra = part == 0 && tid < tail ? score_at(widen(x[extra_place])) : -INFINITY;
+  Vector next[NV];
+  if (tiles > 0) load(first, next);
+  for (int t = 0; t < tiles; ++t, first += kTile) {
     float v[EACH];
-    const bool inside = first >= 0 && first + tile_size <= a.num_values;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const long long at = first + ((long long)i * kThreads + tid) * VE;
-      if (inside || (at >= 0 && at + VE <= a.num_values)) {
-        const Pack<T, VE> p = *reinterpret_cast<const Pack<T, VE>*>(x + at);
+    for (int i = 0; i < EACH; ++i) v[i] = score_at(widen(next[i / VE].at[i % VE]));
+    if (t + 1 < tiles) load(first + kTile, next);
+    float largest = extra;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) v[i * VE + j] = score_at(widen(p.at[j]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < VE; ++j) v[i * VE + j] = at + j >= 0 && at + j < a.num_values ? score_at(widen(x[at + j])) : -INFINITY;
-      }
-    }
-    float largest = v[0];
-#pragma unroll
-    for (int i = 1; i < EACH; ++i) largest = fmaxf(largest, v[i]);
+    for (int i = 0; i < EACH; ++i) largest = fmaxf(largest, v[i]);
     if (a.normalise) {
       constexpr float kLog2e = 1.44269504f;
       if (largest > top) {
@@ -164,37 +175,47 @@ __global__ void __launch_bounds__(kThreads) select_part_kernel(SelectArgs a) {
       }
       const float base = top == -INFINITY ? 0.f : top;
       const float before = sum;
+      sum += __builtin_amdgcn_exp2f((extra - base) * kLog2e);
 #pragma unroll
       for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);
       if (top == INFINITY) {  // (beside an infinite one only the infinite ones count)
-        sum = before;
+        sum = before + (extra == INFINITY ? 1.f : 0.f);
         for (int i = 0; i < EACH; ++i) sum += v[i] == INFINITY ? 1.f : 0.f;
       }
     }
-    if (t == 0) bar = reached_by(largest, a.most, shared);
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) mine += __popcll(__ballot(v[i] >= bar && v[i] > -INFINITY));
+    if (t == 0) bar = reached_by(largest, a.most, INFINITY, shared);
+    uint32_t in = 0;  // which of the thread's scores go to the list
     int at = 0;
-    if (lane == 0 && mine) at = atomicAdd(&filled, mine);
-    at = __shfl(at, 0);
+    if (largest >= bar && largest > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) in |= v[i] >= bar && v[i] > -INFINITY ? 1u << i : 0u;
+      in |= extra >= bar && extra > -INFINITY ? 1u << EACH : 0u;
+      at = atomicAdd(&filled, __popc(in));
+    }
     __syncthreads();
     const int now = filled;
-    auto place = [&](int i) { return (uint32_t)(first + ((long long)(i / VE) * kThreads + tid) * VE + i % VE); };
+    auto place = [&](int i) { return (first + i / VE * kThreads + tid) * VE + i % VE; };
     if (now <= kKept) {
-      if (mine) {
+      if (in) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          const bool in = v[i] >= bar && v[i] > -INFINITY;
-          const unsigned long long with = __ballot(in);
-          if (in) kept[at + __popcll(with & ((1ull << lane) - 1))] = order_key(v[i], place(i));
-          at += __popcll(with);
-        }
+        for (int i = 0; i < EACH; ++i)
+          if (in >> i & 1) kept[at++] = order_key(v[i], (uint32_t)place(i));
+        if (in >> EACH & 1) kept[at++] = order_key(extra, (uint32_t)extra_place);
       }
       have = now;
       __syncthreads();
+      if (t + 1 < tiles && (t == 0 ? have > a.most : have > 2 * kThreads)) {  // what comes after has to beat the worst of the best so far
+        have = keep_best(kept, have, a.most);
+        if (have == a.most) {
+          bar_key = kept[have - 1];
+          bar = key_value(bar_key);
+        }
+        if (tid == 0) filled = have;
+        __syncthreads();
+      }
     } else {
-      for (int i = 0; i < EACH; ++i) {
+#pragma unroll 1
+      for (int i = 0; i <= EACH; ++i) {
         if (i == 0 || have + kThreads > kKept) {
           have = keep_best(kept, have, a.most);
           if (have == a.most) {
@@ -204,16 +225,17 @@ __global__ void __launch_bounds__(kThreads) select_part_kernel(SelectArgs a) {
           if (tid == 0) filled = have;
           __syncthreads();
         }
-        float value = v[0];
-#pragma unroll
-        for (int j = 1; j < EACH; ++j) value = i == j ? v[j] : value;
-        const uint64_t key = order_key(value, place(i));
-        if (value > -INFINITY && key > bar_key) kept[atomicAdd(&filled, 1)] = key;
+        if (in >> i & 1) {
+          const int at_row = i < EACH ? place(i) : extra_place;
+          const uint64_t key = order_key(score_at(widen(x[at_row])), (uint32_t)at_row);
+          if (key > bar_key) kept[atomicAdd(&filled, 1)] = key;
+        }
         __syncthreads();
         have = filled;
         __syncthreads();
       }
     }
+    extra = -INFINITY;
   }
   have = keep_best(kept, have, a.most);
   uint64_t* list = a.lists + (long long)blockIdx.x * a.most;
@@ -251,24 +273,29 @@ __device__ inline double total_value(uint64_t u) {
 __global__ void __launch_bounds__(kThreads) select_merge_kernel(SelectArgs a) {
   __shared__ uint64_t kept_total[kKept], kept_key[kKept];
   __shared__ int kept_beam[kKept];
-  __shared__ uint64_t shared[kWaves];
+  __shared__ uint64_t shared[kThreads];
   __shared__ int filled, first_best;
   extern __shared__ double beam_less[];  // per beam: the logarithm of its sum, and its largest score behind
   double* beam_top = beam_less + a.num_beams;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int per_beam = a.parts * a.most, all = a.num_beams * per_beam;
-  for (int k = tid; k < a.num_beams; k += kThreads) {
+  for (int k = tid >> 6; a.normalise && k < a.num_beams; k += kWaves) {
     const long long row = (long long)b * a.num_beams + k;
-    double top = -INFINITY, sum = 0.0;
-    if (a.normalise && !(a.finished && a.finished[row])) {
-      for (int p = 0; p < a.parts; ++p) top = fmax(top, (double)a.list_top[row * a.parts + p]);
-      for (int p = 0; p < a.parts; ++p) {
-        const double t = a.list_top[row * a.parts + p], s = a.list_sum[row * a.parts + p];
-        if (t > -INFINITY) sum += t == top ? s : s * exp(t - top);
-      }
+    if (a.finished && a.finished[row]) continue;
+    float top = -INFINITY;
+    for (int p = lane; p < a.parts; p += 64) top = fmaxf(top, a.list_top[row * a.parts + p]);
+    for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
+    double sum = 0.0;
+    for (int p = lane; p < a.parts; p += 64) {
+      const float t = a.list_top[row * a.parts + p];
+      const double s = a.list_sum[row * a.parts + p];
+      if (t > -INFINITY) sum += t == top ? s : s * exp((double)t - (double)top);
     }
-    beam_top[k] = top;
-    beam_less[k] = a.normalise ? log(sum) : 0.0;
+    for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
+    if (lane == 0) {
+      beam_top[k] = top;
+      beam_less[k] = log(sum);
+    }
   }
   if (tid == 0) filled = 0;
   __syncthreads();
@@ -289,22 +316,36 @@ __global__ void __launch_bounds__(kThreads) select_merge_kernel(SelectArgs a) {
     }
     return total > -INFINITY ? order_total(total) : 0;
   };
-  uint64_t best = 0;
-  for (int c = tid; c < all; c += kThreads) {
+  constexpr int kHeld = 4;  // candidates of a thread that stay in registers
+  uint64_t best = 0, keys[kHeld], totals[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) keys[i] = tid + i * kThreads < all ? key_of(tid + i * kThreads) : 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    totals[i] = tid + i * kThreads < all ? total_of(tid + i * kThreads, keys[i]) : 0;
+    best = totals[i] > best ? totals[i] : best;
+  }
+  for (int c = tid + kHeld * kThreads; c < all; c += kThreads) {
     const uint64_t t = total_of(c, key_of(c));
     best = t > best ? t : best;
   }
-  const uint64_t bar = reached_by(best, a.num, shared);
-  for (int c = tid; c < all; c += kThreads) {
-    const uint64_t key = key_of(c), t = total_of(c, key);
-    if (t == 0 || t < bar) continue;
+  const uint64_t bar = reached_by(best, a.num, ~(uint64_t)0, shared);
+  auto offer = [&](int c, uint64_t key, uint64_t t) {
+    if (t == 0 || t < bar) return;
     const int at = atomicAdd(&filled, 1);
-    if (at >= kKept) continue;
+    if (at >= kKept) return;
     const int k = c / per_beam;
     kept_total[at] = t;
     kept_key[at] = a.finished && a.finished[(long long)b * a.num_beams + k] ? (uint64_t)(uint32_t)~(uint32_t)a.end : key;
     kept_beam[at] = k;
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) offer(tid + i * kThreads, keys[i], totals[i]);
+  if (best >= bar)
+    for (int c = tid + kHeld * kThreads; c < all; c += kThreads) {
+      const uint64_t key = key_of(c);
+      offer(c, key, total_of(c, key));
+    }
   __syncthreads();
   const int count = filled;
   const long long out = (long long)b * a.num;
@@ -313,6 +354,7 @@ __global__ void __launch_bounds__(kThreads) select_merge_kernel(SelectArgs a) {
       const uint64_t t = kept_total[i], key = kept_key[i];
       const int k = kept_beam[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < count; ++j) {
         const uint64_t other = kept_total[j];
         if (other == t) rank += kept_beam[j] < k || (kept_beam[j] == k && kept_key[j] > key);
@@ -394,20 +436,22 @@ struct ReorderArgs {
 
 template <typename T>
 __device__ inline void copy_or_clear(const unsigned char* from, unsigned char* to, long long bytes, bool there) {
-  constexpr int kAtOnce = 4;
   const long long n = bytes / (long long)sizeof(T), stride = (long long)gridDim.x * 256;
   const T* in = reinterpret_cast<const T*>(from);
   T* out = reinterpret_cast<T*>(to);
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += kAtOnce * stride) {
-    T x[kAtOnce] = {};
-    if (there)
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-        if (i + j * stride < n) x[j] = in[i + j * stride];
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
-      if (i + j * stride < n) out[i + j * stride] = x[j];
+  long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (!there) {
+    for (; i < n; i += stride) out[i] = T{};
+    return;
   }
+  for (; i + 3 * stride < n; i += 4 * stride) {
+    const T a = in[i], b = in[i + stride], c = in[i + 2 * stride], d = in[i + 3 * stride];
+    out[i] = a;
+    out[i + stride] = b;
+    out[i + 2 * stride] = c;
+    out[i + 3 * stride] = d;
+  }
+  for (; i < n; i += stride) out[i] = in[i];
 }
 
 __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
@@ -425,19 +469,21 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   }
 }
 
-// How a selection is spread: tiles of 8 or 32 scores for each thread, and so many workgroups a row.
+// How a selection is spread: tiles of one vector or of 16 scores for each thread, and so many workgroups a row as the machine
+// holds at once (six on a CU: one more would be a second round).
+constexpr int kResident = 6 * 256;
 struct SelectPlan {
   bool small;
   int parts, each;
 };
-static SelectPlan select_plan(int num_batch, int num_beams, int num_values, int num) {
+static SelectPlan select_plan(int type, int num_batch, int num_beams, int num_values, int num) {
   SelectPlan p;
   const long long rows = (long long)num_batch * num_beams;
   const int most = std::min(num, num_values);
   p.small = rows * num_values < 512ll * 8192;
-  const long long tile = kThreads * (p.small ? 8 : 32);
-  const int tiles = (int)((15 + tile - 1 + num_values) / tile);  // (a row may begin inside a vector)
-  const long long wanted = std::min<long long>({(2048 + rows - 1) / rows, 256, std::max<long long>(1, 16384 / ((long long)num_beams * most))});
+  const long long tile = kThreads * (p.small ? 16 / (long long)element_size(type) : 16);
+  const int tiles = (int)((num_values + tile - 1) / tile);
+  const long long wanted = std::min<long long>({std::max<long long>(1, kResident / rows), 256, std::max<long long>(1, 16384 / ((long long)num_beams * most))});
   p.each = (int)((tiles + wanted - 1) / wanted);
   p.parts = (tiles + p.each - 1) / p.each;
   return p;
@@ -463,9 +509,9 @@ using namespace cuhnsw_amd;
 
 extern "C" {
 
-long long cuhnsw_select_beams_workspace(int num_batch, int num_beams, int num_values, int num) {
-  if (num_batch <= 0 || num_beams <= 0 || num_values <= 0 || num <= 0) return 0;
-  return (long long)SelectScratch(nullptr, (long long)num_batch * num_beams, select_plan(num_batch, num_beams, num_values, num).parts,
+long long cuhnsw_select_beams_workspace(int type, int num_batch, int num_beams, int num_values, int num) {
+  if (!known_type(type) || num_batch <= 0 || num_beams <= 0 || num_values <= 0 || num <= 0) return 0;
+  return (long long)SelectScratch(nullptr, (long long)num_batch * num_beams, select_plan(type, num_batch, num_beams, num_values, num).parts,
                                   std::min(num, num_values)).bytes;
 }
 
@@ -475,6 +521,7 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
   return call_guarded([&] {
     want(known_type(type), "select: unknown element type");
     want(num_batch >= 0 && num_beams > 0 && num_values > 0, "select: bad sizes");
+    want(num_values <= 1 << 30, "select: more than 2^30 values");
     want(num > 0 && num <= kMostNum, "select: between 1 and 256 candidates can be asked for");
     want((long long)num_beams * std::min(num, num_values) <= kMostLists, "select: more than 4096 candidates of all beams (beams times candidates asked for)");
     want(num_beams <= kMostBeams, "select: more than 1024 beams");
@@ -482,7 +529,7 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
     if (num_batch == 0) return;
     want(scores && out_totals && out_parents && out_tokens, "select: null argument");
     want(!finished || (end >= 0 && end < num_values), "select: the token that ends a sequence is outside the vocabulary");
-    const SelectPlan p = select_plan(num_batch, num_beams, num_values, num);
+    const SelectPlan p = select_plan(type, num_batch, num_beams, num_values, num);
     const long long rows = (long long)num_batch * num_beams;
     const SelectScratch w(workspace, rows, p.parts, std::min(num, num_values));
     want(workspace && workspace_bytes >= (long long)w.bytes, "select: the workspace is too small");
@@ -493,8 +540,8 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const dim3 grid((unsigned)(rows * p.parts));
-      if (p.small) hipLaunchKernelGGL((select_part_kernel<T, 8>), grid, dim3(kThreads), 0, s, a);
-      else hipLaunchKernelGGL((select_part_kernel<T, 32>), grid, dim3(kThreads), 0, s, a);
+      if (p.small) hipLaunchKernelGGL((select_part_kernel<T, 1>), grid, dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((select_part_kernel<T, sizeof(T)>), grid, dim3(kThreads), 0, s, a);
     });
     hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)num_batch), dim3(kThreads), (size_t)num_beams * 16, s, a);
     HIP_CHECK(hipGetLastError());

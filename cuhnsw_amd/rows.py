@@ -342,7 +342,7 @@ def select_beams(scores, beams, num, normalise=True, finished=None, end=None):
   parents = torch.empty(b, num, dtype=torch.int32, device=device)
   tokens = torch.empty(b, num, dtype=torch.int32, device=device)
   with _on(device):
-    size = _native.select_beams_workspace(b, k, v, num)
+    size = _native.select_beams_workspace(_TYPES[scores.dtype], b, k, v, num)
     work = _workspace(size, device)
     _native.select_beams(scores.data_ptr(), _TYPES[scores.dtype], scores.stride(0), scores.stride(1), b, k, v, _address(beams),
                          _address(finished), 0 if end is None else end, int(bool(normalise)), num, totals.data_ptr(), parents.data_ptr(),

@@ -328,13 +328,13 @@ int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offs
  *   over k and v, largest first; of equal totals (held in 64 bits) the lower k first, then the larger score, then the lower
  *   v.  beams: float32 [num_batch, num_beams] or NULL (zeros).  A NaN counts as -infinity and -infinity is never chosen: places
  *   that are left over say -infinity, -1, -1.  finished (bytes, [num_batch, num_beams]) or NULL: where it is not 0 the beam
- *   has one candidate, token `end` with total beams[b][k].  num_beams <= 1024, num_beams * min(num, num_values) <= 4096.  Results: dense
+ *   has one candidate, token `end` with total beams[b][k].  num_values <= 2^30, num_beams <= 1024, num_beams * min(num, num_values) <= 4096.  Results: dense
  *   [num_batch, num].  (One beam, not normalised: the num nearest neighbours of a matrix of scores.)
  * cuhnsw_reorder_states: for each of num_states arrays to[b][j] = from[b][parents[b][j]], zeros where the parent is outside
  *   [0, num_beams).  Host arrays of device pointers, of byte strides between batch entries and beams, and of the bytes of one
  *   beam's state (contiguous); the results are dense [num_batch, num_picked, bytes] and must not overlap their sources.
  *   Strides of parents in elements. */
-long long cuhnsw_select_beams_workspace(int num_batch, int num_beams, int num_values, int num);
+long long cuhnsw_select_beams_workspace(int type, int num_batch, int num_beams, int num_values, int num);
 int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long long stride_k, int num_batch, int num_beams, int num_values,
                         const float* beams, const unsigned char* finished, int end, int normalise, int num, float* out_totals,
                         int* out_parents, int* out_tokens, void* workspace, long long workspace_bytes, void* stream);
