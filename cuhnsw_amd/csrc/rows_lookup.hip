@@ -15,27 +15,80 @@ __device__ inline long long id_at(const void* ids, int ids_64, long long t) {
   return ids_64 ? reinterpret_cast<const long long*>(ids)[t] : (long long)reinterpret_cast<const int*>(ids)[t];
 }
 
+// A row in whole vectors of VE elements: the last one begins VE before the end, and where that overlaps the one before it both
+// hold the same.  (Global memory takes 16 bytes from and to any address that fits an element, so rows of any length and
+// stride move 16 bytes at a time; rows of fewer elements than a vector go one by one.)
+template <int VE>
+__device__ __host__ inline int vectors_of(int num_dims) {
+  return (num_dims + VE - 1) / VE;
+}
+template <int VE>
+__device__ inline int vector_at(int v, int num_dims) {
+  return min(v * VE, num_dims - VE);
+}
+// lanes that share a row: the power of two that its vectors fill at least half of, a wavefront at most
+inline int lanes_of(int vectors) {
+  int lanes = 1;
+  while (lanes < vectors && lanes < 64) lanes <<= 1;
+  return lanes;
+}
+// f with the elements of a vector as a constant
+template <typename T, typename F>
+void with_vector(int num_dims, F&& f) {
+  constexpr int VE = 16 / sizeof(T);
+  if (num_dims >= VE) f(std::integral_constant<int, VE>());
+  else f(std::integral_constant<int, 1>());
+}
+
 // ---------------------------------------------------------------------------------------------- lookup
-template <typename T, typename U>
+// Bound by memory: each row is fetched once and written once, four rows of a lane's in flight.
+template <typename T, typename U, int VE>
 __global__ void __launch_bounds__(256) lookup_kernel(const T* table, long long num_rows, long long row_stride, int num_dims,
-                                                     const void* ids, int ids_64, long long num_ids, float scale, U* out) {
-  const long long total = num_ids * num_dims;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long t = i / num_dims, d = i - t * num_dims, id = id_at(ids, ids_64, t);
-    out[i] = narrow<U>(id >= 0 && id < num_rows ? scale * widen(table[id * row_stride + d]) : 0.f);
+                                                     const void* ids, int ids_64, long long num_ids, float scale, U* out, int lanes) {
+  constexpr int kAtOnce = 4;
+  const int vectors = vectors_of<VE>(num_dims), lane = threadIdx.x & (lanes - 1);
+  const long long groups = (long long)gridDim.x * (256 / lanes);
+  for (long long t0 = (long long)blockIdx.x * (256 / lanes) + threadIdx.x / lanes; t0 < num_ids; t0 += kAtOnce * groups) {
+    const T* from[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const long long t = t0 + j * groups, id = t < num_ids ? id_at(ids, ids_64, t) : -1;
+      from[j] = id >= 0 && id < num_rows ? table + id * row_stride : nullptr;
+    }
+    for (int v = lane; v < vectors; v += lanes) {
+      const int d = vector_at<VE>(v, num_dims);
+      LoosePack<T, VE> x[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (from[j]) x[j] = *reinterpret_cast<const LoosePack<T, VE>*>(from[j] + d);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const long long t = t0 + j * groups;
+        if (t >= num_ids) break;
+        LoosePack<U, VE> y;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) y.at[e] = narrow<U>(from[j] ? scale * widen(x[j].at[e]) : 0.f);
+        *reinterpret_cast<LoosePack<U, VE>*>(out + t * num_dims + d) = y;
+      }
+    }
   }
 }
 
 void launch_lookup(const LookupArgs& a, hipStream_t stream) {
   if (a.num_ids == 0) return;
-  const long long blocks = std::min<long long>((a.num_ids * a.num_dims + 255) / 256, 1 << 16);
   with_type(a.table_type, [&](auto* t) {
     with_type(a.out_type, [&](auto* u) {
       using T = std::remove_pointer_t<decltype(t)>;
       using U = std::remove_pointer_t<decltype(u)>;
       if constexpr (std::is_same_v<T, U> || std::is_same_v<U, float>) {
-        hipLaunchKernelGGL((lookup_kernel<T, U>), dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const T*>(a.table), a.num_rows,
-                           a.row_stride, a.num_dims, a.ids, a.ids_64, a.num_ids, a.scale, static_cast<U*>(a.out));
+        with_vector<T>(a.num_dims, [&](auto ve) {
+          constexpr int VE = decltype(ve)::value;
+          const int lanes = lanes_of(vectors_of<VE>(a.num_dims)), groups = 256 / lanes;
+          const long long blocks = std::min<long long>((a.num_ids + groups - 1) / groups, 1 << 20);
+          hipLaunchKernelGGL((lookup_kernel<T, U, VE>), dim3((unsigned)(blocks <= 2048 ? blocks : (blocks + 3) / 4)), dim3(256), 0, stream,
+                             static_cast<const T*>(a.table), a.num_rows, a.row_stride, a.num_dims, a.ids, a.ids_64, a.num_ids, a.scale,
+                             static_cast<U*>(a.out), lanes);
+        });
       } else {
         throw std::runtime_error("lookup: the result has the table's type or is float32");
       }
@@ -48,7 +101,7 @@ void launch_lookup(const LookupArgs& a, hipStream_t stream) {
 // A stable sort of (id, place) by id, least significant digit first: places of one id stay in ascending order, so the sums do
 // not depend on how the work was spread.  Ids outside the table take the key num_rows, behind all others.  One pass is two
 // launches: every workgroup counts the digits of its stretch of ids; then each adds up the counts of the others before it,
-// ranks its own ids by ballots among the lanes that hold the same digit, and sends them to their places.
+// and each of its wavefronts ranks a quarter of the stretch by ballots among the lanes that hold the same digit.
 constexpr int kSortThreads = 256, kSortWaves = 4, kSortBlocks = 128, kMostDigits = 2048;
 
 struct SortPlan {
@@ -92,23 +145,31 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortInput in, 
 
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortInput in, int num_ids, int chunk, int shift, int digits, int bits,
                                                                   const int* counts, int* keys, int* places) {
-  __shared__ int next[kMostDigits];               // where the next id with a digit goes
-  __shared__ int wave_count[kSortWaves][kMostDigits];
+  __shared__ int next[kSortWaves][kMostDigits];  // first how many ids a wavefront has with a digit, then where its next one goes
   __shared__ int wave_sum[kSortWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int d = tid; d < digits; d += kSortThreads)
+    for (int w = 0; w < kSortWaves; ++w) next[w][d] = 0;
+  __syncthreads();
+  const int quarter = chunk / kSortWaves, begin = blockIdx.x * chunk + wave * quarter, end = min(num_ids, begin + quarter);
+  for (int i = begin + lane; i < end; i += 64) atomicAdd(&next[wave][(sort_key(in, i) >> shift) & (digits - 1)], 1);
   // ids with a smaller digit anywhere, and with the same digit in an earlier stretch; each thread has consecutive digits
+  constexpr int kDigits = kMostDigits / kSortThreads;
   const int per_thread = (digits + kSortThreads - 1) / kSortThreads;
-  int mine = 0;
-  for (int j = 0; j < per_thread; ++j) {
+  int before[kDigits], mine = 0;
+#pragma unroll
+  for (int j = 0; j < kDigits; ++j) {
     const int d = tid * per_thread + j;
-    if (d >= digits) break;
-    int before = 0, all = 0;
+    before[j] = 0;
+    if (j >= per_thread || d >= digits) continue;
+    int all = 0;
+#pragma unroll 8
     for (int b = 0; b < (int)gridDim.x; ++b) {
       const int n = counts[b * digits + d];
-      before += b < (int)blockIdx.x ? n : 0;
+      before[j] += b < (int)blockIdx.x ? n : 0;
       all += n;
     }
-    next[d] = before + mine;
+    before[j] += mine;
     mine += all;
   }
   int upto = mine;
@@ -120,75 +181,240 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortInput in, 
   __syncthreads();
   int base = upto - mine;
   for (int w = 0; w < wave; ++w) base += wave_sum[w];
-  for (int j = 0; j < per_thread; ++j) {
+#pragma unroll
+  for (int j = 0; j < kDigits; ++j) {
     const int d = tid * per_thread + j;
-    if (d < digits) next[d] += base;
+    if (j >= per_thread || d >= digits) continue;
+    int at = base + before[j];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int n = next[w][d];
+      next[w][d] = at;
+      at += n;
+    }
   }
-  const int begin = blockIdx.x * chunk, end = min(num_ids, begin + chunk);
-  for (int start = begin; start < end; start += kSortThreads) {  // (the same number of rounds for every wavefront)
-    for (int d = tid; d < digits; d += kSortThreads)
-      for (int w = 0; w < kSortWaves; ++w) wave_count[w][d] = 0;
-    __syncthreads();
-    const int i = start + tid;
+  __syncthreads();
+  for (int i = begin + lane; i - lane < end; i += 64) {
     const bool there = i < end;
-    const int key = there ? sort_key(in, i) : 0;
-    const int d = (key >> shift) & (digits - 1);
+    const int key = there ? sort_key(in, i) : 0, d = (key >> shift) & (digits - 1);
     unsigned long long peers = __ballot(there);
     for (int b = 0; b < bits; ++b) {
       const unsigned long long with = __ballot((d >> b) & 1);
       peers &= (d >> b) & 1 ? with : ~with;
     }
     const int rank = __popcll(peers & ((1ull << lane) - 1));
-    if (there && rank == 0) wave_count[wave][d] = __popcll(peers);
-    __syncthreads();
+    int at = 0;
+    if (there && rank == 0) at = atomicAdd(&next[wave][d], __popcll(peers));
+    at = __shfl(at, there ? __ffsll((long long)peers) - 1 : 0) + rank;
     if (there) {
-      int at = next[d] + rank;
-      for (int w = 0; w < wave; ++w) at += wave_count[w][d];
       keys[at] = key;
       places[at] = in.keys ? in.places[i] : i;
     }
-    __syncthreads();
-    for (int x = tid; x < digits; x += kSortThreads)
-      for (int w = 0; w < kSortWaves; ++w) next[x] += wave_count[w][x];
-    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------------------------- gradient
-// first place in [0, n) whose key is at least `key`
+// A workgroup has a stretch of rows and the (key, place) pairs of theirs, in order: out of the sorted list, or, where there
+// are few ids, picked out of all of them and ranked in LDS (one launch, and nothing is sorted).  A row of up to kLong places is a
+// group of lanes' own; the places of a longer one are divided among all groups of the workgroup.  In the sorted list
+// stretches of kLong places of one id have been summed before (grad_long_kernel), so that no row is much longer
+// than that.  Which sum is formed in which order depends on sizes and ids alone.
+constexpr int kLong = 64, kFew = 2048, kMostRows = 128;
+
+// sum of the vector at d over the items [from, to), in order
+template <int VE, typename F>
+__device__ inline void sum_items(int from, int to, F&& item, float (&sum)[VE]) {
+#pragma unroll
+  for (int e = 0; e < VE; ++e) sum[e] = 0.f;
+  int i = from;
+  for (; i + 4 <= to; i += 4) {
+    float x[4][VE];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) item(i + j, x[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) sum[e] += x[j][e];
+  }
+  for (; i < to; ++i) {
+    float x[VE];
+    item(i, x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) sum[e] += x[e];
+  }
+}
+
+// The same by the whole workgroup, a contiguous part of the items for every group of lanes; the first group has the sum.
+// parts: 256 x VE places in LDS.
+template <int VE, typename F>
+__device__ inline void sum_items_together(int items, int lanes, F&& item, float (&sum)[VE], float* parts) {
+  const int groups = 256 / lanes, group = threadIdx.x / lanes, share = (items + groups - 1) / groups;
+  sum_items<VE>(min(items, group * share), min(items, (group + 1) * share), item, sum);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < VE; ++e) parts[threadIdx.x * VE + e] = sum[e];
+  __syncthreads();
+  if (group == 0)
+    for (int g = 1; g < groups; ++g)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) sum[e] += parts[(g * lanes + threadIdx.x) * VE + e];
+}
+
+template <typename T, int VE>
+__device__ inline void fetch(const T* from, float (&x)[VE]) {
+  const LoosePack<T, VE> p = *reinterpret_cast<const LoosePack<T, VE>*>(from);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) x[e] = widen(p.at[e]);
+}
+template <typename U, int VE>
+__device__ inline void store(U* to, const float (&x)[VE], float scale) {
+  LoosePack<U, VE> p;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) p.at[e] = narrow<U>(scale * x[e]);
+  *reinterpret_cast<LoosePack<U, VE>*>(to) = p;
+}
+
+struct GradArgs {
+  const void* grad;
+  long long grad_stride;
+  const void* ids;  // few ids: themselves
+  int ids_64;
+  const int *keys, *places;  // many: in order
+  float* long_sums;          // [num_ids / kLong, num_dims]: sums of the stretches that are one id's alone
+  int num_ids, num_rows, num_dims;
+  float scale;
+  void* out;
+  int lanes, rows;  // lanes that share a row, rows of a workgroup
+};
+
+template <typename T, int VE>
+__global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
+  __shared__ float parts[256 * VE];
+  const int first = blockIdx.x * kLong, key = a.keys[first];
+  if (key >= a.num_rows || a.keys[first + kLong - 1] != key) return;
+  const int lane = threadIdx.x & (a.lanes - 1), vectors = vectors_of<VE>(a.num_dims);
+  const T* grad = static_cast<const T*>(a.grad);
+  for (int v0 = 0; v0 < vectors; v0 += a.lanes) {
+    const int d = vector_at<VE>(min(v0 + lane, vectors - 1), a.num_dims);
+    float sum[VE];
+    sum_items_together<VE>(kLong, a.lanes, [&](int i, float (&x)[VE]) { fetch<T, VE>(grad + (long long)a.places[first + i] * a.grad_stride + d, x); },
+                           sum, parts);
+    if (threadIdx.x < a.lanes) store<float, VE>(a.long_sums + (long long)blockIdx.x * a.num_dims + d, sum, 1.f);
+  }
+}
+
+// by a wavefront: the first place in [0, n) whose key is at least `key`
 __device__ inline int lower_bound(const int* keys, int n, int key) {
-  int low = 0, high = n;
-  while (low < high) {
-    const int mid = (low + high) >> 1;
-    if (keys[mid] < key) low = mid + 1;
-    else high = mid;
+  const int lane = threadIdx.x & 63;
+  int low = 0, size = n;
+  while (size > 0) {
+    const int step = (size + 63) / 64, at = low + (lane + 1) * step - 1;
+    const int less = __popcll(__ballot((lane + 1) * (long long)step <= size && keys[at] < key));
+    low += less * step;
+    size = min(step - 1, size - less * step);
   }
   return low;
 }
 
-template <typename T, typename U>
-__global__ void __launch_bounds__(256) grad_kernel(const T* grad, long long grad_stride, const int* keys, const int* places, int num_ids,
-                                                   int num_rows, int num_dims, float scale, U* out) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= num_rows) return;
-  const int begin = lower_bound(keys, num_ids, row), end = lower_bound(keys, num_ids, row + 1);
-  for (int d = lane; d < num_dims; d += 64) {
-    float sum = 0.f;
-    for (int i = begin; i < end; ++i) sum += widen(grad[(long long)places[i] * grad_stride + d]);
-    out[(long long)row * num_dims + d] = narrow<U>(scale * sum);
+template <typename T, typename U, int VE, bool FEW>
+__global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
+  __shared__ int first[kMostRows], last[kMostRows];
+  __shared__ int bounds[2];
+  __shared__ float parts[256 * VE];
+  __shared__ uint64_t picked[FEW ? kFew : 1];
+  __shared__ int in_order[FEW ? kFew : 1];
+  const int tid = threadIdx.x, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.num_rows - row0);
+  for (int r = tid; r < rows; r += 256) first[r] = last[r] = 0;
+  if (FEW) {
+    if (tid == 0) bounds[0] = 0;
+    __syncthreads();
+    for (int i = tid; i < a.num_ids; i += 256) {
+      const long long r = id_at(a.ids, a.ids_64, i) - row0;
+      if (r >= 0 && r < rows) picked[atomicAdd(&bounds[0], 1)] = (uint64_t)r << 32 | (uint32_t)i;
+    }
+    __syncthreads();
+    const int count = bounds[0];
+    for (int i = tid; i < count; i += 256) {
+      const uint64_t mine = picked[i];
+      int rank = 0, same = 0, under = 0;
+      for (int j = 0; j < count; ++j) {
+        const uint64_t other = picked[j];
+        rank += other < mine;
+        same += other >> 32 == mine >> 32;
+        under += other >> 32 < mine >> 32;
+      }
+      in_order[rank] = (int)(uint32_t)mine;
+      if (rank == under) {
+        first[mine >> 32] = under;
+        last[mine >> 32] = under + same;
+      }
+    }
+  } else {
+    if (tid < 128) {
+      const int at = lower_bound(a.keys, a.num_ids, tid < 64 ? row0 : row0 + rows);
+      if ((tid & 63) == 0) bounds[tid >> 6] = at;
+    }
+    __syncthreads();
+    for (int i = bounds[0] + tid; i < bounds[1]; i += 256) {
+      const int key = a.keys[i];
+      if (i == bounds[0] || a.keys[i - 1] != key) first[key - row0] = i;
+      if (i + 1 == bounds[1] || a.keys[i + 1] != key) last[key - row0] = i + 1;
+    }
+  }
+  __syncthreads();
+  const T* grad = static_cast<const T*>(a.grad);
+  U* out = static_cast<U*>(a.out) + (long long)row0 * a.num_dims;
+  const int lane = tid & (a.lanes - 1), groups = 256 / a.lanes, vectors = vectors_of<VE>(a.num_dims);
+  bool any_long = false;
+  for (int r = tid / a.lanes; r < rows; r += groups) {
+    const int from = first[r], to = last[r];
+    if (to - from > kLong) {
+      any_long = true;
+      continue;
+    }
+    for (int v = lane; v < vectors; v += a.lanes) {
+      const int d = vector_at<VE>(v, a.num_dims);
+      float sum[VE];
+      sum_items<VE>(from, to, [&](int i, float (&x)[VE]) {
+        fetch<T, VE>(grad + (long long)(FEW ? in_order[i] : a.places[i]) * a.grad_stride + d, x);
+      }, sum);
+      store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
+    }
+  }
+  if (!__syncthreads_or(any_long)) return;
+  for (int r = 0; r < rows; ++r) {
+    const int from = first[r], to = last[r];
+    if (to - from <= kLong) continue;
+    // its places up to the first whole stretch, the whole stretches, the places behind them
+    const int whole = FEW ? to : (from + kLong - 1) / kLong, ends = FEW ? to : to / kLong;
+    const int head = FEW ? to - from : whole * kLong - from, stretches = FEW ? 0 : ends - whole, tail = FEW ? 0 : to - ends * kLong;
+    for (int v0 = 0; v0 < vectors; v0 += a.lanes) {
+      const int d = vector_at<VE>(min(v0 + lane, vectors - 1), a.num_dims);
+      float sum[VE];
+      sum_items_together<VE>(head + stretches + tail, a.lanes, [&](int i, float (&x)[VE]) {
+        if (!FEW && i >= head && i < head + stretches) {
+          fetch<float, VE>(a.long_sums + (long long)(whole + i - head) * a.num_dims + d, x);
+        } else {
+          const int at = i < head ? from + i : ends * kLong + i - head - stretches;
+          fetch<T, VE>(grad + (long long)(FEW ? in_order[at] : a.places[at]) * a.grad_stride + d, x);
+        }
+      }, sum, parts);
+      if (tid < a.lanes) store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
+    }
   }
 }
 
 struct GradScratch {
   int *keys[2], *places[2], *counts;
+  float* long_sums;
   size_t bytes;
-  GradScratch(void* memory, long long num_ids, const SortPlan& p) {
+  GradScratch(void* memory, long long num_ids, int num_dims, const SortPlan& p) {
     WorkspaceParts s(memory);
     for (int i = 0; i < 2; ++i) {
       keys[i] = s.part<int>((size_t)num_ids);
       places[i] = s.part<int>((size_t)num_ids);
     }
     counts = s.part<int>((size_t)p.blocks << p.bits);
+    long_sums = s.part<float>((size_t)(num_ids / kLong) * num_dims);
     bytes = s.used();
   }
 };
@@ -211,8 +437,8 @@ int cuhnsw_lookup_rows(const void* table, int table_type, long long num_rows, lo
 }
 
 long long cuhnsw_lookup_grad_workspace(long long num_ids, long long num_rows, int num_dims) {
-  if (num_ids <= 0 || num_rows <= 0 || num_dims <= 0) return 0;
-  return (long long)GradScratch(nullptr, num_ids, sort_plan(num_ids, num_rows)).bytes;
+  if (num_ids <= kFew || num_ids > 1 << 30 || num_rows <= 0 || num_rows >= 0x7fffffff || num_dims <= 0) return 0;
+  return (long long)GradScratch(nullptr, num_ids, num_dims, sort_plan(num_ids, num_rows)).bytes;
 }
 
 int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stride, const void* ids, int ids_64, long long num_ids,
@@ -226,10 +452,20 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
     want(num_ids == 0 || (grad && ids), "lookup gradient: null argument");
     if (num_rows == 0) return;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int *keys = nullptr, *places = nullptr;
-    if (num_ids > 0) {
+    GradArgs g{};
+    g.grad = grad;
+    g.grad_stride = grad_stride;
+    g.ids = ids;
+    g.ids_64 = ids_64;
+    g.num_ids = (int)num_ids;
+    g.num_rows = (int)num_rows;
+    g.num_dims = num_dims;
+    g.scale = scale;
+    g.out = out;
+    const bool few = num_ids <= kFew;
+    if (!few) {
       const SortPlan p = sort_plan(num_ids, num_rows);
-      const GradScratch w(workspace, num_ids, p);
+      const GradScratch w(workspace, num_ids, num_dims, p);
       want(workspace && workspace_bytes >= (long long)w.bytes, "lookup gradient: the workspace is too small");
       for (int pass = 0; pass < p.passes; ++pass) {
         const SortInput in{ids, ids_64, (int)num_rows, pass ? w.keys[(pass - 1) & 1] : nullptr, pass ? w.places[(pass - 1) & 1] : nullptr};
@@ -238,16 +474,30 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
         hipLaunchKernelGGL(sort_place_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, in, (int)num_ids, p.chunk, pass * p.bits, 1 << p.bits,
                            p.bits, w.counts, w.keys[pass & 1], w.places[pass & 1]);
       }
-      keys = w.keys[(p.passes - 1) & 1];
-      places = w.places[(p.passes - 1) & 1];
+      g.keys = w.keys[(p.passes - 1) & 1];
+      g.places = w.places[(p.passes - 1) & 1];
+      g.long_sums = w.long_sums;
     }
     with_type(grad_type, [&](auto* t) {
       with_type(out_type, [&](auto* u) {
         using T = std::remove_pointer_t<decltype(t)>;
         using U = std::remove_pointer_t<decltype(u)>;
         if constexpr (std::is_same_v<T, U> || std::is_same_v<T, float>) {
-          hipLaunchKernelGGL((grad_kernel<T, U>), dim3((unsigned)((num_rows + 3) / 4)), dim3(256), 0, s, static_cast<const T*>(grad), grad_stride,
-                             keys, places, (int)num_ids, (int)num_rows, num_dims, scale, static_cast<U*>(out));
+          with_vector<T>(num_dims, [&](auto ve) {
+            constexpr int VE = decltype(ve)::value;
+            g.lanes = lanes_of(vectors_of<VE>(num_dims));
+            // rows for about 32 KB in and out, whole turns of the groups of lanes
+            const int groups = 256 / g.lanes;
+            const long long bytes = (long long)num_dims * (sizeof(U) + sizeof(T) * (num_ids / num_rows));
+            g.rows = (int)std::min<long long>(kMostRows, std::max<long long>(groups, 32768 / bytes / groups * groups));
+            const dim3 grid((unsigned)((num_rows + g.rows - 1) / g.rows));
+            if (few) {
+              hipLaunchKernelGGL((grad_kernel<T, U, VE, true>), grid, dim3(256), 0, s, g);
+            } else {
+              hipLaunchKernelGGL((grad_long_kernel<T, VE>), dim3((unsigned)(num_ids / kLong)), dim3(256), 0, s, g);
+              hipLaunchKernelGGL((grad_kernel<T, U, VE, false>), grid, dim3(256), 0, s, g);
+            }
+          });
         } else {
           throw std::runtime_error("lookup gradient: the gradient has the table's type or is float32");
         }

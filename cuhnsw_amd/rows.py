@@ -133,8 +133,8 @@ def lookup_grad(grad, ids, num_rows, scale=1.0, dtype=None):
   """The gradient of lookup with respect to its table: [num_rows, dims], row v the sum of scale * grad[t] over the places
   t with ids[t] = v.
 
-  grad: [*ids.shape, dims].  The sums run over the places in ascending order, in 32 bits, rounded once to `dtype`
-  (grad's own, or any where grad is float32): the same inputs give the same bits, whatever the device does meanwhile."""
+  grad: [*ids.shape, dims].  The sums are formed in 32 bits, in an order that depends on the ids alone, and rounded once to
+  `dtype` (grad's own, or any where grad is float32): the same inputs give the same bits."""
   _tensor(grad, "grad")
   _tensor(ids, "ids", types=_IDS)
   scale = _number(scale, "scale")

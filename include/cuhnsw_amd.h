@@ -295,8 +295,8 @@ int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, vo
  *
  * cuhnsw_lookup_rows: out[t] = scale * table[ids[t]], zeros where ids[t] is outside [0, num_rows) (padded places: -1).
  *   ids: int32, or int64 with ids_64; out: dense [num_ids, num_dims], of the table's type or float32.
- * cuhnsw_lookup_rows_grad: out[v] = scale * sum of grad[t] over the t with ids[t] = v, t ascending: the result does not
- *   depend on how the work was spread.  All of out is written: dense [num_rows, num_dims], of the gradient's type, or
+ * cuhnsw_lookup_rows_grad: out[v] = scale * sum of grad[t] over the t with ids[t] = v.  In which order the sum is formed
+ *   depends on the sizes and the ids alone: the same call gives the same bits.  All of out is written: dense [num_rows, num_dims], of the gradient's type, or
  *   of any where that is float32.  num_ids <= 2^30, num_rows < 2^31 - 1. */
 int cuhnsw_lookup_rows(const void* table, int table_type, long long num_rows, long long row_stride, int num_dims, const void* ids,
                        int ids_64, long long num_ids, float scale, void* out, int out_type, void* stream);

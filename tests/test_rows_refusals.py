@@ -76,6 +76,7 @@ def test_scratch_sizes():
   l = capi.load()
   for args in ((0, 5, 3), (5, 0, 3), (5, 5, 0), (-1, 5, 3)):
     assert l.cuhnsw_lookup_grad_workspace(*args) == 0
+  assert l.cuhnsw_lookup_grad_workspace(2048, 1000, 50) == 0    # (few ids need none)
   assert l.cuhnsw_lookup_grad_workspace(100000, 1183514, 50) >= 100000 * 8
   assert l.cuhnsw_select_beams_workspace(0, 0, 1, 1, 1) == 0
   assert l.cuhnsw_select_beams_workspace(3, 1, 1, 1, 1) == 0
