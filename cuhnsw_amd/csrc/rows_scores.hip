@@ -83,8 +83,9 @@ void launch_pack(const PackArgs& a, hipStream_t stream) {
 // float16 is one plane.  Products are summed in 32 bits per group of elements; the group's scale is applied to that sum, so
 // no weight is ever rounded.  Offsets meet the group's sum of query elements.
 //
-// Queries are laid out once per call (prepare_kernel) as the lanes want them: for a tile of up to 16 queries and a unit of 32 elements,
-// 16 bytes for every quarter of a unit and query, in the order in which the codes of a word come apart.
+// Queries are laid out as the lanes want them: for a tile of 16 queries and a unit of 32 elements, 16 bytes for every quarter of the
+// unit and query.  That is a launch of its own (prepare_kernel), or, where they are few and short, every workgroup's first
+// step, into its LDS.
 constexpr int kTile = 16, kUnit = 32, kRowTiles = 4;  // queries or rows of a matrix product, elements of it; row tiles of a wavefront
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -106,49 +107,66 @@ struct ScoresArgs {
   int out_type;
   long long out_stride;
   int padded_units;        // units that the planes hold: the last are zero
-  _Float16* planes;        // [planes][query tile][unit][quarter][query][8]
+  _Float16* planes;        // [planes][query tile][unit][quarter][16][8]
   size_t plane;            // elements of one plane
-  int* exponents;          // [num_queries]: what the scores are to be scaled by
+  int* exponents;          // of every query: what its scores are to be scaled by
   float* sums;             // [query tile][group][16]: sums of the groups' elements
   int query_blocks, row_blocks, split;
 };
 
+// Power of two that takes the largest magnitude of a query to [2^14, 2^15): the exponent of the largest element, by the whole
+// workgroup.  A float16 query stays as it is, and one that is zero or not finite too.
+template <typename T>
+__device__ inline int exponent_of(const T* q, int num_dims, float* per_wave) {
+  if (std::is_same_v<T, _Float16>) return 14;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  float most = 0.f;
+  for (int k = tid; k < num_dims; k += threads) {
+    const float x = fabsf(widen(q[k]));
+    most = x < INFINITY ? fmaxf(most, x) : INFINITY;  // (a NaN too)
+  }
+  for (int step = 32; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
+  if ((tid & 63) == 0) per_wave[tid >> 6] = most;
+  __syncthreads();
+  for (int w = 0; w < threads / 64; ++w) most = fmaxf(most, per_wave[w]);
+  __syncthreads();
+  return most > 0.f && most < INFINITY ? ilogbf(most) : 14;
+}
+// Eight elements, a quarter of a unit, in the order in which the codes of a word come apart: 0 4 1 5 2 6 3 7.
+template <typename T>
+__device__ inline void planes_of_eight(const T* q, int first, int num_dims, int exponent, half8_t& high, half8_t& low) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = first + (e & 1) * 4 + (e >> 1);
+    const float x = k < num_dims ? ldexpf(widen(q[k]), 14 - exponent) : 0.f;
+    high[e] = (_Float16)x;
+    low[e] = (_Float16)(x - (float)high[e]);
+  }
+}
+template <typename T>
+__device__ inline float sum_of_group(const T* q, int g, const ScoresArgs& a, int exponent) {
+  float sum = 0.f;
+  for (int k = g * a.group; k < min(a.num_dims, (g + 1) * a.group); ++k) sum += ldexpf(widen(q[k]), -exponent);
+  return sum;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) prepare_kernel(ScoresArgs a, int planes) {
-  __shared__ float largest[4];
-  const int m = blockIdx.x, tid = threadIdx.x;
-  const T* q = static_cast<const T*>(a.queries) + m * a.query_stride;
-  int exponent = 14;
-  if (!std::is_same_v<T, _Float16>) {
-    float most = 0.f;
-    for (int k = tid; k < a.num_dims; k += 256) most = fmaxf(most, fabsf(widen(q[k])));
-    for (int step = 32; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
-    if ((tid & 63) == 0) largest[tid >> 6] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
-    if (most > 0.f && most < INFINITY) exponent = ilogbf(most);
-  }
+  __shared__ float per_wave[4];
+  const int m = blockIdx.x, tid = threadIdx.x, tile = m / kTile, i = m % kTile;
+  const bool there = m < a.num_queries;  // (the last tile is filled up with zeros)
+  const T* q = static_cast<const T*>(a.queries) + (there ? m : 0) * a.query_stride;
+  const int num_dims = there ? a.num_dims : 0, exponent = exponent_of(q, num_dims, per_wave);
   if (tid == 0) a.exponents[m] = exponent;
-  const int tile = m / kTile, i = m % kTile, in_tile = min(kTile, a.num_queries - tile * kTile);
   _Float16* to = a.planes + (size_t)tile * kTile * a.padded_units * kUnit;
-  for (int w = tid; w < a.padded_units * 4; w += 256) {  // eight elements: a quarter of a unit
+  for (int w = tid; w < a.padded_units * 4; w += 256) {
     half8_t high, low;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int k = w * 8 + (e & 1) * 4 + (e >> 1);  // (0 4 1 5 2 6 3 7)
-      const float x = k < a.num_dims ? ldexpf(widen(q[k]), 14 - exponent) : 0.f;
-      high[e] = (_Float16)x;
-      low[e] = (_Float16)(x - (float)high[e]);
-    }
-    *reinterpret_cast<half8_t*>(to + ((size_t)w * in_tile + i) * 8) = high;
-    if (planes == 2) *reinterpret_cast<half8_t*>(to + a.plane + ((size_t)w * in_tile + i) * 8) = low;
+    planes_of_eight(q, w * 8, num_dims, exponent, high, low);
+    *reinterpret_cast<half8_t*>(to + ((size_t)w * kTile + i) * 8) = high;
+    if (planes == 2) *reinterpret_cast<half8_t*>(to + a.plane + ((size_t)w * kTile + i) * 8) = low;
   }
   if (a.offsets)
-    for (int g = tid; g < a.groups; g += 256) {
-      float sum = 0.f;
-      for (int k = g * a.group; k < min(a.num_dims, (g + 1) * a.group); ++k) sum += ldexpf(widen(q[k]), -exponent);
-      a.sums[((size_t)tile * a.groups + g) * kTile + i] = sum;
-    }
+    for (int g = tid; g < a.groups; g += 256) a.sums[((size_t)tile * a.groups + g) * kTile + i] = there ? sum_of_group(q, g, a, exponent) : 0.f;
 }
 
 // The eight codes of a word, less 8 or as they are, as float16, in the order 0 4 1 5 2 6 3 7: a code behind the exponent of 1024
@@ -166,195 +184,397 @@ __device__ inline half8_t codes_of(uint32_t word) {
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A wavefront has 64 rows (four tiles of 16) and MT tiles of queries, and goes over the elements in chunks of UC units; `split`
-// wavefronts of the workgroup share the chunks of the same rows.  A load of 16 bytes brings a unit's codes to a lane: four such
-// slots, one for each quarter of the wavefront, are different units of one row tile, or on short rows of several.  Four lane
-// exchanges then give every quarter its quarter of each slot, so one matrix product covers one unit, inside one group.
-template <int UC, int GU, int MT, int PLANES, bool CENTRED>
-__global__ void __launch_bounds__(512) scores_kernel(ScoresArgs a) {
+// the four words of a unit's codes in each of four slots, quarter by quarter of the wavefront -> the quarters' own words of
+// each slot
+__device__ inline void exchange(uint4 words, uint32_t (&slots)[4]) {
+  const auto ac = __builtin_amdgcn_permlane32_swap(words.x, words.z, false, false);
+  const auto bd = __builtin_amdgcn_permlane32_swap(words.y, words.w, false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(ac[0], bd[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(ac[1], bd[1], false, false);
+  slots[0] = lo[0];
+  slots[1] = lo[1];
+  slots[2] = hi[0];
+  slots[3] = hi[1];
+}
+
+__device__ inline void store_score(const ScoresArgs& a, int query, long long row, float sum, int exponent) {
+  float y = a.alpha * ldexpf(sum, exponent);
+  if (a.bias) y += a.bias[row];
+  const long long at = query * a.out_stride + row;
+  if (a.out_type == TYPE_F32) static_cast<float*>(a.out)[at] = y;
+  else if (a.out_type == TYPE_F16) static_cast<_Float16*>(a.out)[at] = (_Float16)y;
+  else static_cast<bf16*>(a.out)[at] = narrow<bf16>(y);
+}
+
+// Few queries: bound by the rows' codes.  A wavefront has 64 rows (four tiles of 16) and one tile of queries, and goes over the
+// elements in chunks of UC units, two chunks ahead; `split` wavefronts of the workgroup share the chunks of the same rows.
+// A load of 16 bytes brings a unit's codes to a lane: four such slots, one for each quarter of the wavefront, are
+// different units of one row tile, or on short rows of several.  Four lane exchanges then give every quarter its quarter
+// of each slot, so one matrix product covers one unit, inside one group.
+// OWN: the workgroup lays the queries out itself (at most 16), else T is not looked at.
+template <typename T, int UC, int GU, int PLANES, bool CENTRED, bool OWN>
+__global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
   constexpr int kGroups = (UC + GU - 1) / GU;  // of a chunk
-  constexpr int kAcc = kRowTiles * MT;
-  extern __shared__ float4_t partial[];  // [split - 1][row block][kAcc][64]
+  extern __shared__ __align__(16) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int j = lane & 15, c = lane >> 4;
-  // the query blocks of the same rows one after the other on the same chiplet, whose L2 then holds the rows
-  const int turn = blockIdx.x >> 3, per_block = waves / a.split;
-  const int block = (turn / a.query_blocks) * 8 + (blockIdx.x & 7), tile0 = (turn % a.query_blocks) * MT;
+  const int per_block = waves / a.split, block = blockIdx.x / a.query_blocks, tile = blockIdx.x % a.query_blocks;
   const int share = wave % a.split, in_block = wave / a.split;
-  const long long row0 = ((long long)block * per_block + in_block) * (kRowTiles * kTile);
-  const bool there = row0 < a.num_rows;
-  float4_t acc[kRowTiles][MT];
+  const long long row0 = ((long long)block * per_block + in_block) * (kRowTiles * kTile), last_row = a.num_rows - 1;
+  const int chunks = (a.units + UC - 1) / UC, per_share = (chunks + a.split - 1) / a.split;
+  const int chunk0 = share * per_share, chunk1 = row0 <= last_row ? min(chunks, chunk0 + per_share) : 0;
+
+  struct Stage {
+    uint4 words[UC];
+    uint16_t scales[kRowTiles][kGroups], offsets[kRowTiles][kGroups];
+    half8_t query[UC][PLANES];
+  };
+  const unsigned char* from[UC];
+  int unit_of[UC];
 #pragma unroll
-  for (int t = 0; t < kRowTiles; ++t)
+  for (int i = 0; i < UC; ++i) {
+    const int slot = 4 * i + c;
+    unit_of[i] = slot % UC;
+    from[i] = a.codes + min(row0 + slot / UC * kTile + j, last_row) * ((long long)a.units * 16);
+  }
+  long long groups_of[kRowTiles];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
-  if (there) {
-    const size_t row_bytes = (size_t)a.units * 16;
-    const unsigned char* from[UC];
-    int unit_of[UC];
+  for (int t = 0; t < kRowTiles; ++t) groups_of[t] = min(row0 + t * kTile + j, last_row) * a.groups;
+  const _Float16* planes = a.planes + (size_t)tile * kTile * a.padded_units * kUnit + lane * 8;
+  auto load = [&](Stage& s, int chunk) {
+    if (chunk >= chunk1) return;
 #pragma unroll
-    for (int i = 0; i < UC; ++i) {
-      const int slot = 4 * i + c;
-      const long long row = min(row0 + slot / UC * kTile + j, (long long)a.num_rows - 1);
-      unit_of[i] = slot % UC;
-      from[i] = a.codes + row * row_bytes;
-    }
-    long long groups_of[kRowTiles];
+    for (int i = 0; i < UC; ++i) s.words[i] = *reinterpret_cast<const uint4*>(from[i] + min(chunk * UC + unit_of[i], a.units - 1) * 16);
 #pragma unroll
-    for (int t = 0; t < kRowTiles; ++t) groups_of[t] = min(row0 + t * kTile + j, (long long)a.num_rows - 1) * a.groups;
-    const _Float16* query_of[MT];
-    int in_tile[MT];
-    const float* sum_of[MT];
+    for (int t = 0; t < kRowTiles; ++t)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int tile = min(tile0 + m, (a.num_queries - 1) / kTile);
-      in_tile[m] = min(kTile, a.num_queries - tile * kTile);
-      query_of[m] = a.planes + (size_t)tile * kTile * a.padded_units * kUnit + (c * in_tile[m] + min(j, in_tile[m] - 1)) * 8;
-      sum_of[m] = a.sums + (size_t)tile * a.groups * kTile + c * 4;
-    }
-    const int chunks = (a.units + UC - 1) / UC, per_share = (chunks + a.split - 1) / a.split;
-    const int chunk0 = share * per_share, chunk1 = min(chunks, chunk0 + per_share);
-    uint4 next[UC];
-    auto load = [&](int chunk) {
-#pragma unroll
-      for (int i = 0; i < UC; ++i)
-        next[i] = *reinterpret_cast<const uint4*>(from[i] + min(chunk * UC + unit_of[i], a.units - 1) * 16);
-    };
-    if (chunk0 < chunk1) load(chunk0);
-    for (int chunk = chunk0; chunk < chunk1; ++chunk) {
-      uint4 now[UC];
-#pragma unroll
-      for (int i = 0; i < UC; ++i) now[i] = next[i];
-      float scale[kRowTiles][kGroups], offset[kRowTiles][kGroups];
-#pragma unroll
-      for (int t = 0; t < kRowTiles; ++t)
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const int at = min(chunk * UC / GU + g, a.groups - 1);
-          scale[t][g] = half_bits(a.scales[groups_of[t] + at], a.scale_bf16) * 0x1p-14f;
-          if (!CENTRED) offset[t][g] = half_bits(a.offsets[groups_of[t] + at], a.scale_bf16);
-        }
-      half8_t query[UC][MT][PLANES];
+      for (int g = 0; g < kGroups; ++g) {
+        const long long at = groups_of[t] + min(chunk * UC / GU + g, a.groups - 1);
+        s.scales[t][g] = a.scales[at];
+        if (!CENTRED) s.offsets[t][g] = a.offsets[at];
+      }
+    if (!OWN)
 #pragma unroll
       for (int u = 0; u < UC; ++u)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int p = 0; p < PLANES; ++p) s.query[u][p] = *reinterpret_cast<const half8_t*>(planes + p * a.plane + (size_t)(chunk * UC + u) * 512);
+  };
+  Stage even, odd;
+  load(even, chunk0);
+  load(odd, chunk0 + 1);
+
+  // (own queries) [planes][unit][quarter][query][8], then the groups' sums [group][16], then the exponents
+  const int own_queries = min(kTile, a.num_queries), own_plane = a.padded_units * kUnit * own_queries;
+  _Float16* own = reinterpret_cast<_Float16*>(lds);
+  float* own_sums = reinterpret_cast<float*>(own + (size_t)PLANES * own_plane);
+  int* own_exponents = reinterpret_cast<int*>(own_sums + (CENTRED ? 0 : kTile * a.groups));
+  float* per_wave = reinterpret_cast<float*>(own_exponents + kTile);
+  float4_t* partial = reinterpret_cast<float4_t*>(OWN ? reinterpret_cast<unsigned char*>(per_wave + 8) : lds);
+  if (OWN) {
+    for (int i = 0; i < own_queries; ++i) {
+      const T* q = static_cast<const T*>(a.queries) + i * a.query_stride;
+      const int exponent = exponent_of(q, a.num_dims, per_wave);
+      if (threadIdx.x == 0) own_exponents[i] = exponent;
+      for (int w = threadIdx.x; w < a.padded_units * 4; w += blockDim.x) {
+        half8_t high, low;
+        planes_of_eight(q, w * 8, a.num_dims, exponent, high, low);
+        *reinterpret_cast<half8_t*>(own + ((size_t)w * own_queries + i) * 8) = high;
+        if (PLANES == 2) *reinterpret_cast<half8_t*>(own + own_plane + ((size_t)w * own_queries + i) * 8) = low;
+      }
+      if (!CENTRED)
+        for (int g = threadIdx.x; g < a.groups; g += blockDim.x) own_sums[g * kTile + i] = sum_of_group(q, g, a, exponent);
+    }
+    __syncthreads();
+  }
+
+  float4_t acc[kRowTiles];
 #pragma unroll
-          for (int p = 0; p < PLANES; ++p)
-            query[u][m][p] = *reinterpret_cast<const half8_t*>(query_of[m] + p * a.plane + (size_t)(chunk * UC + u) * 32 * in_tile[m]);
-      if (chunk + 1 < chunk1) load(chunk + 1);
-      float4_t temp[MT];
+  for (int t = 0; t < kRowTiles; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  auto use = [&](const Stage& s, int chunk) {
+    half8_t query[UC][PLANES];
 #pragma unroll
-      for (int i = 0; i < UC; ++i) {
-        const auto ac = __builtin_amdgcn_permlane32_swap(now[i].x, now[i].z, false, false);
-        const auto bd = __builtin_amdgcn_permlane32_swap(now[i].y, now[i].w, false, false);
-        const auto lo = __builtin_amdgcn_permlane16_swap(ac[0], bd[0], false, false);
-        const auto hi = __builtin_amdgcn_permlane16_swap(ac[1], bd[1], false, false);
-        const uint32_t slots[4] = {lo[0], lo[1], hi[0], hi[1]};
+    for (int u = 0; u < UC; ++u)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int slot = 4 * i + q, t = slot / UC, u = slot % UC;
-          const half8_t codes = codes_of<CENTRED>(slots[q]);
+      for (int p = 0; p < PLANES; ++p)
+        query[u][p] = OWN ? *reinterpret_cast<const half8_t*>(own + p * own_plane + (((chunk * UC + u) * 4 + c) * own_queries + min(j, own_queries - 1)) * 8)
+                          : s.query[u][p];
+    float4_t temp;
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            if (u % GU == 0) temp[m] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < UC; ++i) {
+      uint32_t slots[4];
+      exchange(s.words[i], slots);
 #pragma unroll
-            for (int p = PLANES - 1; p >= 0; --p)
-              temp[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(query[u][m][p], codes, temp[m], 0, 0, 0);
-            if (u % GU == GU - 1 || u == UC - 1) {
-              const float s = scale[t][u / GU];
+      for (int q = 0; q < 4; ++q) {
+        const int slot = 4 * i + q, t = slot / UC, u = slot % UC;
+        const half8_t codes = codes_of<CENTRED>(slots[q]);
+        if (u % GU == 0) temp = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int r = 0; r < 4; ++r) acc[t][m][r] = fmaf(s, temp[m][r], acc[t][m][r]);
-              if (!CENTRED && chunk * UC / GU + u / GU < a.groups) {
-                const float4_t x = *reinterpret_cast<const float4_t*>(sum_of[m] + (chunk * UC / GU + u / GU) * kTile);
-                const float o = offset[t][u / GU];
+        for (int p = PLANES - 1; p >= 0; --p) temp = __builtin_amdgcn_mfma_f32_16x16x32_f16(query[u][p], codes, temp, 0, 0, 0);
+        if (u % GU != GU - 1 && u != UC - 1) continue;
+        const float scale = half_bits(s.scales[t][u / GU], a.scale_bf16) * 0x1p-14f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[t][m][r] = fmaf(o, x[r], acc[t][m][r]);
-              }
-            }
-          }
+        for (int r = 0; r < 4; ++r) acc[t][r] = fmaf(scale, temp[r], acc[t][r]);
+        if (!CENTRED) {  // (behind the last group there is nothing)
+          const int group = chunk * UC / GU + u / GU, held = min(group, a.groups - 1);
+          const float* sums = OWN ? own_sums + held * kTile : a.sums + ((size_t)tile * a.groups + held) * kTile;
+          const float4_t x = *reinterpret_cast<const float4_t*>(sums + c * 4);
+          const float offset = group == held ? half_bits(s.offsets[t][u / GU], a.scale_bf16) : 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[t][r] = fmaf(offset, x[r], acc[t][r]);
         }
       }
+    }
+  };
+  for (int chunk = chunk0; chunk < chunk1; chunk += 2) {
+    use(even, chunk);
+    load(even, chunk + 2);
+    if (chunk + 1 < chunk1) {
+      use(odd, chunk + 1);
+      load(odd, chunk + 3);
     }
   }
   if (a.split > 1) {
     if (share > 0)
 #pragma unroll
-      for (int t = 0; t < kAcc; ++t) partial[(((share - 1) * per_block + in_block) * kAcc + t) * 64 + lane] = acc[t / MT][t % MT];
+      for (int t = 0; t < kRowTiles; ++t) partial[(((share - 1) * per_block + in_block) * kRowTiles + t) * 64 + lane] = acc[t];
     __syncthreads();
     if (share > 0) return;
     for (int s = 0; s < a.split - 1; ++s)
 #pragma unroll
-      for (int t = 0; t < kAcc; ++t) acc[t / MT][t % MT] += partial[((s * per_block + in_block) * kAcc + t) * 64 + lane];
+      for (int t = 0; t < kRowTiles; ++t) acc[t] += partial[((s * per_block + in_block) * kRowTiles + t) * 64 + lane];
   }
-  if (!there) return;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int r = 0; r < 4; ++r) {
+    const int query = tile * kTile + c * 4 + r;
+    if (query >= a.num_queries) continue;
+    const int exponent = OWN ? own_exponents[c * 4 + r] : a.exponents[query];
+#pragma unroll
+    for (int t = 0; t < kRowTiles; ++t)
+      if (row0 + t * kTile + j <= last_row) store_score(a, query, row0 + t * kTile + j, acc[t][r], exponent);
+  }
+}
+
+// Many queries: a workgroup of four wavefronts has 256 rows and MT tiles of queries.  The queries' planes of a chunk go through LDS
+// (straight from memory, the next chunk's while this one is at work), so four wavefronts share what they read of them; a
+// unit's planes stay in registers over the wavefront's four row tiles.
+template <int UC, int GU, int MT, int PLANES, bool CENTRED>
+__global__ void __launch_bounds__(256, 2) scores_many_kernel(ScoresArgs a) {
+  constexpr int kGroups = (UC + GU - 1) / GU, kPieces = UC * MT * PLANES;  // pieces of 1 KB: what a wavefront reads at once
+  __shared__ half8_t queries[2][kPieces][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, c = lane >> 4;
+  // the query blocks of the same rows one after the other on the same chiplet, whose L2 then holds the rows
+  const int turn = blockIdx.x >> 3, block = (turn / a.query_blocks) * 8 + (blockIdx.x & 7), tile0 = (turn % a.query_blocks) * MT;
+  if (block >= a.row_blocks) return;
+  const int last_tile = (a.num_queries - 1) / kTile, chunks = (a.units + UC - 1) / UC;
+  const long long row0 = (long long)block * (4 * kRowTiles * kTile) + wave * (kRowTiles * kTile), last_row = a.num_rows - 1;
+
+  const unsigned char* from[UC];
+  int unit_of[UC];
+#pragma unroll
+  for (int i = 0; i < UC; ++i) {
+    const int slot = 4 * i + c;
+    unit_of[i] = slot % UC;
+    from[i] = a.codes + min(row0 + slot / UC * kTile + j, last_row) * ((long long)a.units * 16);
+  }
+  long long groups_of[kRowTiles];
+#pragma unroll
+  for (int t = 0; t < kRowTiles; ++t) groups_of[t] = min(row0 + t * kTile + j, last_row) * a.groups;
+  uint4 words[UC];
+  uint16_t scales[kRowTiles][kGroups], offsets[kRowTiles][kGroups];
+  auto load = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < UC; ++i) words[i] = *reinterpret_cast<const uint4*>(from[i] + min(chunk * UC + unit_of[i], a.units - 1) * 16);
+#pragma unroll
+    for (int t = 0; t < kRowTiles; ++t)
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const long long at = groups_of[t] + min(chunk * UC / GU + g, a.groups - 1);
+        scales[t][g] = a.scales[at];
+        if (!CENTRED) offsets[t][g] = a.offsets[at];
+      }
+  };
+  // piece (u, m, p) of a chunk: 64 x 16 bytes that lie in a row in the planes
+  auto bring = [&](int chunk, int buffer) {
+    for (int piece = wave; piece < kPieces; piece += 4) {
+      const int p = piece % PLANES, m = piece / PLANES % MT, u = piece / PLANES / MT;
+      const _Float16* there = a.planes + p * a.plane + ((size_t)min(tile0 + m, last_tile) * a.padded_units + chunk * UC + u) * (kTile * kUnit) + lane * 8;
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(there)),
+                                       (__attribute__((address_space(3))) void*)&queries[buffer][piece][0], 16, 0, 0);
+    }
+  };
+  float4_t acc[kRowTiles][MT];
+#pragma unroll
+  for (int t = 0; t < kRowTiles; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
+  bring(0, 0);
+  load(0);
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    // (what was brought is in LDS once every wavefront has waited for its own loads)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t word[kRowTiles][UC];
+#pragma unroll
+    for (int i = 0; i < UC; ++i) {
+      uint32_t slots[4];
+      exchange(words[i], slots);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) word[(4 * i + q) / UC][(4 * i + q) % UC] = slots[q];
+    }
+    float scale[kRowTiles][kGroups], offset[kRowTiles][kGroups];
+#pragma unroll
+    for (int t = 0; t < kRowTiles; ++t)
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        scale[t][g] = half_bits(scales[t][g], a.scale_bf16) * 0x1p-14f;
+        // (behind the last group there is nothing)
+        offset[t][g] = CENTRED || chunk * UC / GU + g >= a.groups ? 0.f : half_bits(offsets[t][g], a.scale_bf16);
+      }
+    if (chunk + 1 < chunks) {
+      bring(chunk + 1, (chunk + 1) & 1);
+      load(chunk + 1);
+    }
+    float4_t temp[kRowTiles][MT];
+#pragma unroll
+    for (int u = 0; u < UC; ++u) {
+      half8_t query[MT][PLANES];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) query[m][p] = queries[chunk & 1][(u * MT + m) * PLANES + p][lane];
+      const int group = min(chunk * UC / GU + u / GU, a.groups - 1);
+      float4_t x[MT];
+      if (!CENTRED && (u % GU == GU - 1 || u == UC - 1))
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          x[m] = *reinterpret_cast<const float4_t*>(a.sums + ((size_t)min(tile0 + m, last_tile) * a.groups + group) * kTile + c * 4);
+#pragma unroll
+      for (int t = 0; t < kRowTiles; ++t) {
+        const half8_t codes = codes_of<CENTRED>(word[t][u]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (u % GU == 0) temp[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = PLANES - 1; p >= 0; --p) temp[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(query[m][p], codes, temp[t][m], 0, 0, 0);
+          if (u % GU != GU - 1 && u != UC - 1) continue;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[t][m][r] = fmaf(scale[t][u / GU], temp[t][m][r], acc[t][m][r]);
+          if (!CENTRED)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][m][r] = fmaf(offset[t][u / GU], x[m][r], acc[t][m][r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int query = (tile0 + m) * kTile + c * 4 + r;
       if (query >= a.num_queries) continue;
       const int exponent = a.exponents[query];
 #pragma unroll
-      for (int t = 0; t < kRowTiles; ++t) {
-        const long long row = row0 + t * kTile + j;
-        if (row >= a.num_rows) continue;
-        float y = a.alpha * ldexpf(acc[t][m][r], exponent);
-        if (a.bias) y += a.bias[row];
-        const long long at = query * a.out_stride + row;
-        if (a.out_type == TYPE_F32) static_cast<float*>(a.out)[at] = y;
-        else if (a.out_type == TYPE_F16) static_cast<_Float16*>(a.out)[at] = (_Float16)y;
-        else static_cast<bf16*>(a.out)[at] = narrow<bf16>(y);
-      }
+      for (int t = 0; t < kRowTiles; ++t)
+        if (row0 + t * kTile + j <= last_row) store_score(a, query, row0 + t * kTile + j, acc[t][m][r], exponent);
+    }
+}
+
+inline int units_of(int num_dims) { return (num_dims + kUnit - 1) / kUnit; }
+inline int planes_of(int query_type) { return query_type == TYPE_F32 ? 2 : 1; }
+
+// How a call is spread.
+struct ScoresPlan {
+  int chunk, padded_units, planes, groups;  // units of a chunk; of a row, with the units that fill the last chunk up
+  int query_tiles;                          // of a workgroup; 0: few queries
+  bool own;                                 // few queries, laid out by the workgroups themselves
+  int split, waves, query_blocks, row_blocks;
+  size_t lds;
+  ScoresPlan(long long num_rows, int num_dims, int group, int query_type, int num_queries) {
+    const int units = units_of(num_dims), tiles = (num_queries + kTile - 1) / kTile;
+    planes = planes_of(query_type);
+    groups = (num_dims + group - 1) / group;
+    query_blocks = (tiles + 3) / 4;
+    const long long blocks = (num_rows + 255) / 256;
+    query_tiles = tiles > 1 && blocks * query_blocks >= 256 ? (tiles + query_blocks - 1) / query_blocks : 0;
+    own = false;
+    lds = 0;
+    if (query_tiles) {
+      chunk = units <= 2 ? 2 : 4;
+      split = 1;
+      waves = 4;
+      row_blocks = (int)blocks;
+    } else {
+      chunk = std::min(units, 4);
+      query_blocks = tiles;
+      const long long row_waves = (num_rows + 63) / 64;
+      const int chunks = (units + chunk - 1) / chunk;
+      split = 1;
+      while (split < 8 && split < chunks && row_waves * tiles * split < 4096) split *= 2;
+      waves = std::max(4, split);
+      row_blocks = (int)((row_waves + waves / split - 1) / (waves / split));
+    }
+    padded_units = (units + chunk - 1) / chunk * chunk;
+    if (!query_tiles) {
+      const size_t laid_out = (size_t)padded_units * kUnit * std::min(num_queries, kTile) * planes * 2 + (size_t)groups * kTile * 4 + kTile * 4 + 32;
+      own = tiles == 1 && laid_out <= 32768;
+      lds = (own ? (laid_out + 15) / 16 * 16 : 0) + (size_t)(split > 1 ? (split - 1) * (waves / split) : 0) * kRowTiles * 64 * sizeof(float4_t);
     }
   }
-}
+};
 
 struct ScoresScratch {
   _Float16* planes;
   int* exponents;
   float* sums;
   size_t plane, bytes;
-  ScoresScratch(void* memory, int num_queries, int padded_units, int planes_wanted, int groups) {
+  ScoresScratch(void* memory, int num_queries, const ScoresPlan& p) {
     WorkspaceParts s(memory);
-    plane = (size_t)num_queries * padded_units * kUnit;
-    planes = s.part<_Float16>(plane * planes_wanted);
-    exponents = s.part<int>((size_t)num_queries);
-    sums = s.part<float>((size_t)(num_queries + kTile - 1) / kTile * kTile * groups);
+    const size_t queries = p.own ? 0 : (size_t)(num_queries + kTile - 1) / kTile * kTile;
+    plane = queries * p.padded_units * kUnit;
+    planes = s.part<_Float16>(plane * p.planes);
+    exponents = s.part<int>(queries);
+    sums = s.part<float>(queries * p.groups);
     bytes = s.used();
   }
 };
-inline int units_of(int num_dims) { return (num_dims + kUnit - 1) / kUnit; }
-inline int chunk_of(int units) { return std::min(units, 4); }
-inline int padded_units_of(int units) { return (units + chunk_of(units) - 1) / chunk_of(units) * chunk_of(units); }
-inline int planes_of(int query_type) { return query_type == TYPE_F32 ? 2 : 1; }
+
+template <typename T, int UC, int GU, int PLANES, bool OWN>
+void launch_few(const ScoresArgs& a, const ScoresPlan& p, hipStream_t stream) {
+  const long long grid = (long long)a.row_blocks * a.query_blocks;
+  want(grid <= 0x7fffffff, "scores: too many rows and queries");
+  if (a.offsets) hipLaunchKernelGGL((scores_few_kernel<T, UC, GU, PLANES, false, OWN>), dim3((unsigned)grid), dim3(64 * p.waves), p.lds, stream, a);
+  else hipLaunchKernelGGL((scores_few_kernel<T, UC, GU, PLANES, true, OWN>), dim3((unsigned)grid), dim3(64 * p.waves), p.lds, stream, a);
+}
+template <int UC, int GU>
+void launch_few_of(const ScoresArgs& a, const ScoresPlan& p, int query_type, hipStream_t stream) {
+  if (p.own && query_type == TYPE_F32) launch_few<float, UC, GU, 2, true>(a, p, stream);
+  else if (p.own && query_type == TYPE_F16) launch_few<_Float16, UC, GU, 1, true>(a, p, stream);
+  else if (p.own) launch_few<bf16, UC, GU, 1, true>(a, p, stream);
+  else if (p.planes == 2) launch_few<float, UC, GU, 2, false>(a, p, stream);
+  else launch_few<float, UC, GU, 1, false>(a, p, stream);
+}
 
 template <int UC, int GU, int MT, int PLANES>
-void launch_scores(const ScoresArgs& a, int waves, hipStream_t stream) {
-  const dim3 grid((unsigned)(((long long)a.row_blocks + 7) / 8 * 8 * a.query_blocks));
-  const size_t lds = a.split > 1 ? (size_t)(a.split - 1) * (waves / a.split) * kRowTiles * MT * 64 * sizeof(float4_t) : 0;
-  if (a.offsets) hipLaunchKernelGGL((scores_kernel<UC, GU, MT, PLANES, false>), grid, dim3(64 * waves), lds, stream, a);
-  else hipLaunchKernelGGL((scores_kernel<UC, GU, MT, PLANES, true>), grid, dim3(64 * waves), lds, stream, a);
+void launch_many(const ScoresArgs& a, hipStream_t stream) {
+  const long long grid = ((long long)a.row_blocks + 7) / 8 * 8 * a.query_blocks;
+  want(grid <= 0x7fffffff, "scores: too many rows and queries");
+  if (a.offsets) hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+}
+template <int UC, int GU, int MT>
+void launch_many_of(const ScoresArgs& a, const ScoresPlan& p, hipStream_t stream) {
+  if (p.planes == 2) launch_many<UC, GU, MT, 2>(a, stream);
+  else launch_many<UC, GU, MT, 1>(a, stream);
 }
 
 template <int UC, int GU>
-void plan_scores(ScoresArgs& a, int planes, hipStream_t stream) {
-  const int tiles = (a.num_queries + kTile - 1) / kTile, mt = tiles == 1 ? 1 : tiles == 2 ? 2 : 4;
-  const long long blocks = ((long long)a.num_rows + kRowTiles * kTile - 1) / (kRowTiles * kTile);
-  const int chunks = (a.units + UC - 1) / UC;
-  a.query_blocks = (tiles + mt - 1) / mt;
-  a.split = 1;
-  while (mt < 4 && a.split < 8 && a.split < chunks && blocks * a.query_blocks * a.split < 4096) a.split *= 2;
-  const int waves = std::max(4, a.split);
-  a.row_blocks = (int)((blocks + waves / a.split - 1) / (waves / a.split));
-  auto with_planes = [&](auto mts) {
-    constexpr int MT = decltype(mts)::value;
-    if (planes == 2) launch_scores<UC, GU, MT, 2>(a, waves, stream);
-    else launch_scores<UC, GU, MT, 1>(a, waves, stream);
-  };
-  if (mt == 1) with_planes(std::integral_constant<int, 1>());
-  else if (mt == 2) with_planes(std::integral_constant<int, 2>());
-  else with_planes(std::integral_constant<int, 4>());
+void launch_scores(const ScoresArgs& a, const ScoresPlan& p, int query_type, hipStream_t stream) {
+  if constexpr (UC == 2 || UC == 4) {
+    if (p.query_tiles == 4) return launch_many_of<UC, GU, 4>(a, p, stream);
+    if (p.query_tiles == 3) return launch_many_of<UC, GU, 3>(a, p, stream);
+    if (p.query_tiles > 0) return launch_many_of<UC, GU, 2>(a, p, stream);
+  }
+  launch_few_of<UC, GU>(a, p, query_type, stream);
 }
 
 }  // namespace cuhnsw_amd
@@ -384,7 +604,7 @@ int cuhnsw_pack_rows(const void* rows, int type, long long row_stride, long long
 
 long long cuhnsw_packed_scores_workspace(long long num_rows, int num_dims, int group, int query_type, int num_queries) {
   if (num_rows <= 0 || num_dims <= 0 || group <= 0 || !known_type(query_type) || num_queries <= 0) return 0;
-  return (long long)ScoresScratch(nullptr, num_queries, padded_units_of(units_of(num_dims)), planes_of(query_type), (num_dims + group - 1) / group).bytes;
+  return (long long)ScoresScratch(nullptr, num_queries, ScoresPlan(num_rows, num_dims, group, query_type, num_queries)).bytes;
 }
 
 int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offsets, int scale_type, long long num_rows, int num_dims,
@@ -418,24 +638,28 @@ int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offs
     a.out = out;
     a.out_type = out_type;
     a.out_stride = out_stride;
-    a.padded_units = padded_units_of(a.units);
-    const int planes = planes_of(query_type);
-    const ScoresScratch w(workspace, num_queries, a.padded_units, planes, a.groups);
-    want(workspace && workspace_bytes >= (long long)w.bytes, "scores: the workspace is too small");
+    const ScoresPlan p(num_rows, num_dims, group, query_type, num_queries);
+    a.padded_units = p.padded_units;
+    a.query_blocks = p.query_blocks;
+    a.row_blocks = p.row_blocks;
+    a.split = p.split;
+    const ScoresScratch w(workspace, num_queries, p);
+    want(w.bytes == 0 || (workspace && workspace_bytes >= (long long)w.bytes), "scores: the workspace is too small");
     a.planes = w.planes;
     a.plane = w.plane;
     a.exponents = w.exponents;
     a.sums = w.sums;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    with_type(query_type, [&](auto* t) {
-      using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL(prepare_kernel<T>, dim3((unsigned)num_queries), dim3(256), 0, s, a, planes);
-    });
-    const int uc = chunk_of(a.units), gu = group / kUnit;
-    if (uc == 1) plan_scores<1, 1>(a, planes, s);
-    else if (uc == 2) gu == 1 ? plan_scores<2, 1>(a, planes, s) : plan_scores<2, 2>(a, planes, s);
-    else if (uc == 3) gu == 1 ? plan_scores<3, 1>(a, planes, s) : gu == 2 ? plan_scores<3, 2>(a, planes, s) : plan_scores<3, 4>(a, planes, s);
-    else gu == 1 ? plan_scores<4, 1>(a, planes, s) : gu == 2 ? plan_scores<4, 2>(a, planes, s) : plan_scores<4, 4>(a, planes, s);
+    if (!p.own)
+      with_type(query_type, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        hipLaunchKernelGGL(prepare_kernel<T>, dim3((unsigned)((num_queries + kTile - 1) / kTile * kTile)), dim3(256), 0, s, a, p.planes);
+      });
+    const int gu = group / kUnit;
+    if (p.chunk == 1) launch_scores<1, 1>(a, p, query_type, s);
+    else if (p.chunk == 2) gu == 1 ? launch_scores<2, 1>(a, p, query_type, s) : launch_scores<2, 2>(a, p, query_type, s);
+    else if (p.chunk == 3) gu == 1 ? launch_scores<3, 1>(a, p, query_type, s) : gu == 2 ? launch_scores<3, 2>(a, p, query_type, s) : launch_scores<3, 4>(a, p, query_type, s);
+    else gu == 1 ? launch_scores<4, 1>(a, p, query_type, s) : gu == 2 ? launch_scores<4, 2>(a, p, query_type, s) : launch_scores<4, 4>(a, p, query_type, s);
     HIP_CHECK(hipGetLastError());
   });
 }
