@@ -111,7 +111,7 @@ struct ScoresArgs {
   size_t plane;            // elements of one plane
   int* exponents;          // of every query: what its scores are to be scaled by
   float* sums;             // [query tile][group][16]: sums of the groups' elements
-  int query_blocks, row_blocks, split;
+  int query_blocks, row_blocks, split, blocks_each;
 };
 
 // Power of two that takes the largest magnitude of a query to [2^14, 2^15): the exponent of the largest element, by the whole
@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(256) prepare_kernel(ScoresArgs a, int planes) 
 // is 1024 more (16 times the code behind it for every other one), and what is too much goes off exactly.
 template <bool CENTRED>
 __device__ inline half8_t codes_of(uint32_t word) {
-  constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u, k1024 = 0x64006400u;
+  constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+  uint32_t k1024 = 0x64006400u;
+  asm("" : "+v"(k1024));  // (in a vector register: one instruction takes the bits out and puts the exponent in)
   const half2_t low = CENTRED ? half2_t{-1032.f16, -1032.f16} : half2_t{-1024.f16, -1024.f16};
   const half2_t high = CENTRED ? half2_t{-72.f16, -72.f16} : half2_t{-64.f16, -64.f16}, sixteenth = {0.0625f16, 0.0625f16};
   const uint32_t next = word >> 8;
@@ -182,6 +184,59 @@ __device__ inline half8_t codes_of(uint32_t word) {
   const half2_t c = __builtin_bit_cast(half2_t, (next & kLow) | k1024) + low;
   const half2_t d = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (next & kHigh) | k1024), sixteenth, high);
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Scales or offsets of a chunk's N groups, two in a word.
+typedef uint32_t loose32 __attribute__((aligned(2)));
+typedef uint64_t loose64 __attribute__((aligned(2)));
+template <int N>
+struct Groups {
+  uint32_t words[(N + 1) / 2];
+  __device__ uint16_t operator[](int g) const { return (uint16_t)(words[g / 2] >> (g % 2 * 16)); }
+};
+// from group `first` on, at once where they are all the row's own (the others are not looked at)
+template <int N>
+__device__ inline Groups<N> load_groups(const uint16_t* row, int first, int groups) {
+  Groups<N> x;
+  const uint16_t* from = row + first;
+  if (first + N <= groups) {
+    if constexpr (N == 1) {
+      x.words[0] = from[0];
+    } else if constexpr (N == 2) {
+      x.words[0] = *reinterpret_cast<const loose32*>(from);
+    } else if constexpr (N == 3) {
+      x.words[0] = *reinterpret_cast<const loose32*>(from);
+      x.words[1] = from[2];
+    } else {
+      const uint64_t both = *reinterpret_cast<const loose64*>(from);
+      x.words[0] = (uint32_t)both;
+      x.words[1] = (uint32_t)(both >> 32);
+    }
+  } else {
+    for (int w = 0; w < (N + 1) / 2; ++w)
+      x.words[w] = (uint32_t)row[min(first + 2 * w, groups - 1)] | (uint32_t)row[min(first + 2 * w + 1, groups - 1)] << 16;
+  }
+  return x;
+}
+// of every quarter of the wavefront its word, to all lanes
+__device__ inline void from_quarters(uint32_t word, uint32_t (&all)[4]) {
+  const auto halves = __builtin_amdgcn_permlane32_swap(word, word, false, false);
+  const auto low = __builtin_amdgcn_permlane16_swap(halves[0], halves[0], false, false);
+  const auto high = __builtin_amdgcn_permlane16_swap(halves[1], halves[1], false, false);
+  all[0] = low[0];
+  all[1] = low[1];
+  all[2] = high[0];
+  all[3] = high[1];
+}
+template <int N>
+__device__ inline void from_quarters(const Groups<N>& x, Groups<N> (&all)[4]) {
+#pragma unroll
+  for (int w = 0; w < (N + 1) / 2; ++w) {
+    uint32_t words[4];
+    from_quarters(x.words[w], words);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) all[q].words[w] = words[q];
+  }
 }
 
 // the four words of a unit's codes in each of four slots, quarter by quarter of the wavefront -> the quarters' own words of
@@ -197,17 +252,55 @@ __device__ inline void exchange(uint4 words, uint32_t (&slots)[4]) {
   slots[3] = hi[1];
 }
 
-__device__ inline void store_score(const ScoresArgs& a, int query, long long row, float sum, int exponent) {
-  float y = a.alpha * ldexpf(sum, exponent);
-  if (a.bias) y += a.bias[row];
-  const long long at = query * a.out_stride + row;
-  if (a.out_type == TYPE_F32) static_cast<float*>(a.out)[at] = y;
-  else if (a.out_type == TYPE_F16) static_cast<_Float16*>(a.out)[at] = (_Float16)y;
-  else static_cast<bf16*>(a.out)[at] = narrow<bf16>(y);
+// A lane's scores: RT rows one after the other from `row` on, for four queries of every tile.
+template <int RT, int MT>
+__device__ inline void store_scores(const ScoresArgs& a, const float4_t (&acc)[RT][MT], int tile0, int c, long long row, const int* exponents = nullptr) {
+  const int rows = (int)min((long long)RT, a.num_rows - row);
+  float bias[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) bias[t] = a.bias && t < rows ? a.bias[row + t] : 0.f;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int query = (tile0 + m) * kTile + c * 4 + r;
+      if (query < a.num_queries && rows > 0) {
+        const int exponent = exponents ? exponents[c * 4 + r] : a.exponents[query];
+        const long long at = query * a.out_stride + row;
+        LoosePack<float, RT> y;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) y.at[t] = a.alpha * ldexpf(acc[t][m][r], exponent) + bias[t];
+        if (a.out_type == TYPE_F32) {
+          float* to = static_cast<float*>(a.out) + at;
+          if (rows == RT) *reinterpret_cast<LoosePack<float, RT>*>(to) = y;
+          else
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+              if (t < rows) to[t] = y.at[t];
+        } else {
+          uint16_t* to = static_cast<uint16_t*>(a.out) + at;
+          uint32_t words[RT / 2];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            const uint16_t bits = a.out_type == TYPE_BF16 ? narrow<bf16>(y.at[t]).bits : __builtin_bit_cast(uint16_t, (_Float16)y.at[t]);
+            words[t / 2] = t % 2 ? words[t / 2] | (uint32_t)bits << 16 : bits;
+          }
+          if (rows == RT) {
+            if constexpr (RT == 2) *reinterpret_cast<loose32*>(to) = words[0];
+            else *reinterpret_cast<loose64*>(to) = (uint64_t)words[RT / 2 - 1] << 32 | words[0];
+          } else {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+              if (t < rows) to[t] = (uint16_t)(words[t / 2] >> (t % 2 * 16));
+          }
+        }
+      }
+    }
 }
 
 // Few queries: bound by the rows' codes.  A wavefront has 64 rows (four tiles of 16) and one tile of queries, and goes over the
 // elements in chunks of UC units, two chunks ahead; `split` wavefronts of the workgroup share the chunks of the same rows.
+// Rows 4 j to 4 j + 3 are lane j's in the four tiles, so that it stores them together.
 // A load of 16 bytes brings a unit's codes to a lane: four such slots, one for each quarter of the wavefront, are
 // different units of one row tile, or on short rows of several.  Four lane exchanges then give every quarter its quarter
 // of each slot, so one matrix product covers one unit, inside one group.
@@ -226,7 +319,7 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
 
   struct Stage {
     uint4 words[UC];
-    uint16_t scales[kRowTiles][kGroups], offsets[kRowTiles][kGroups];
+    Groups<kGroups> scales, offsets;  // of row tile c's row of the lane
     half8_t query[UC][PLANES];
   };
   const unsigned char* from[UC];
@@ -235,24 +328,16 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
   for (int i = 0; i < UC; ++i) {
     const int slot = 4 * i + c;
     unit_of[i] = slot % UC;
-    from[i] = a.codes + min(row0 + slot / UC * kTile + j, last_row) * ((long long)a.units * 16);
+    from[i] = a.codes + min(row0 + j * kRowTiles + slot / UC, last_row) * ((long long)a.units * 16);
   }
-  long long groups_of[kRowTiles];
-#pragma unroll
-  for (int t = 0; t < kRowTiles; ++t) groups_of[t] = min(row0 + t * kTile + j, last_row) * a.groups;
+  const long long groups_of = min(row0 + j * kRowTiles + c, last_row) * a.groups;
   const _Float16* planes = a.planes + (size_t)tile * kTile * a.padded_units * kUnit + lane * 8;
   auto load = [&](Stage& s, int chunk) {
     if (chunk >= chunk1) return;
 #pragma unroll
     for (int i = 0; i < UC; ++i) s.words[i] = *reinterpret_cast<const uint4*>(from[i] + min(chunk * UC + unit_of[i], a.units - 1) * 16);
-#pragma unroll
-    for (int t = 0; t < kRowTiles; ++t)
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const long long at = groups_of[t] + min(chunk * UC / GU + g, a.groups - 1);
-        s.scales[t][g] = a.scales[at];
-        if (!CENTRED) s.offsets[t][g] = a.offsets[at];
-      }
+    s.scales = load_groups<kGroups>(a.scales + groups_of, chunk * UC / GU, a.groups);
+    if (!CENTRED) s.offsets = load_groups<kGroups>(a.offsets + groups_of, chunk * UC / GU, a.groups);
     if (!OWN)
 #pragma unroll
       for (int u = 0; u < UC; ++u)
@@ -287,9 +372,9 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
     __syncthreads();
   }
 
-  float4_t acc[kRowTiles];
+  float4_t acc[kRowTiles][1];
 #pragma unroll
-  for (int t = 0; t < kRowTiles; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < kRowTiles; ++t) acc[t][0] = float4_t{0.f, 0.f, 0.f, 0.f};
   auto use = [&](const Stage& s, int chunk) {
     half8_t query[UC][PLANES];
 #pragma unroll
@@ -298,6 +383,9 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
       for (int p = 0; p < PLANES; ++p)
         query[u][p] = OWN ? *reinterpret_cast<const half8_t*>(own + p * own_plane + (((chunk * UC + u) * 4 + c) * own_queries + min(j, own_queries - 1)) * 8)
                           : s.query[u][p];
+    Groups<kGroups> scales[kRowTiles], offsets[kRowTiles];
+    from_quarters(s.scales, scales);
+    if (!CENTRED) from_quarters(s.offsets, offsets);
     float4_t temp;
 #pragma unroll
     for (int i = 0; i < UC; ++i) {
@@ -311,16 +399,16 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
 #pragma unroll
         for (int p = PLANES - 1; p >= 0; --p) temp = __builtin_amdgcn_mfma_f32_16x16x32_f16(query[u][p], codes, temp, 0, 0, 0);
         if (u % GU != GU - 1 && u != UC - 1) continue;
-        const float scale = half_bits(s.scales[t][u / GU], a.scale_bf16) * 0x1p-14f;
+        const float scale = half_bits(scales[t][u / GU], a.scale_bf16) * 0x1p-14f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[t][r] = fmaf(scale, temp[r], acc[t][r]);
+        for (int r = 0; r < 4; ++r) acc[t][0][r] = fmaf(scale, temp[r], acc[t][0][r]);
         if (!CENTRED) {  // (behind the last group there is nothing)
           const int group = chunk * UC / GU + u / GU, held = min(group, a.groups - 1);
           const float* sums = OWN ? own_sums + held * kTile : a.sums + ((size_t)tile * a.groups + held) * kTile;
           const float4_t x = *reinterpret_cast<const float4_t*>(sums + c * 4);
-          const float offset = group == held ? half_bits(s.offsets[t][u / GU], a.scale_bf16) : 0.f;
+          const float offset = group == held ? half_bits(offsets[t][u / GU], a.scale_bf16) : 0.f;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[t][r] = fmaf(offset, x[r], acc[t][r]);
+          for (int r = 0; r < 4; ++r) acc[t][0][r] = fmaf(offset, x[r], acc[t][0][r]);
         }
       }
     }
@@ -336,147 +424,149 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
   if (a.split > 1) {
     if (share > 0)
 #pragma unroll
-      for (int t = 0; t < kRowTiles; ++t) partial[(((share - 1) * per_block + in_block) * kRowTiles + t) * 64 + lane] = acc[t];
+      for (int t = 0; t < kRowTiles; ++t) partial[(((share - 1) * per_block + in_block) * kRowTiles + t) * 64 + lane] = acc[t][0];
     __syncthreads();
     if (share > 0) return;
     for (int s = 0; s < a.split - 1; ++s)
 #pragma unroll
-      for (int t = 0; t < kRowTiles; ++t) acc[t] += partial[((s * per_block + in_block) * kRowTiles + t) * 64 + lane];
+      for (int t = 0; t < kRowTiles; ++t) acc[t][0] += partial[((s * per_block + in_block) * kRowTiles + t) * 64 + lane];
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int query = tile * kTile + c * 4 + r;
-    if (query >= a.num_queries) continue;
-    const int exponent = OWN ? own_exponents[c * 4 + r] : a.exponents[query];
-#pragma unroll
-    for (int t = 0; t < kRowTiles; ++t)
-      if (row0 + t * kTile + j <= last_row) store_score(a, query, row0 + t * kTile + j, acc[t][r], exponent);
-  }
+  store_scores<kRowTiles, 1>(a, acc, tile, c, row0 + j * kRowTiles, OWN ? own_exponents : nullptr);
 }
 
-// Many queries: a workgroup of four wavefronts has 256 rows and MT tiles of queries.  The queries' planes of a chunk go through LDS
-// (straight from memory, the next chunk's while this one is at work), so four wavefronts share what they read of them; a
-// unit's planes stay in registers over the wavefront's four row tiles.
+// Many queries: a workgroup of eight wavefronts has 256 rows, 32 for each wavefront, and goes over `blocks_each` blocks of MT
+// tiles of queries, chunk by chunk of UC units.  The queries' planes of a chunk go through LDS (straight from memory, the
+// next chunk's while this one is at work), so eight wavefronts share what they read of them; a unit's planes stay in
+// registers over the wavefront's two row tiles.  Rows 2 j and 2 j + 1 are lane j's in the two tiles, so that it stores them
+// together.
 template <int UC, int GU, int MT, int PLANES, bool CENTRED>
-__global__ void __launch_bounds__(256, 2) scores_many_kernel(ScoresArgs a) {
+__global__ void __launch_bounds__(512, 4) scores_many_kernel(ScoresArgs a) {
+  constexpr int RT = 2, kLoads = UC * RT / 4;
   constexpr int kGroups = (UC + GU - 1) / GU, kPieces = UC * MT * PLANES;  // pieces of 1 KB: what a wavefront reads at once
   __shared__ half8_t queries[2][kPieces][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, c = lane >> 4;
-  // the query blocks of the same rows one after the other on the same chiplet, whose L2 then holds the rows
-  const int turn = blockIdx.x >> 3, block = (turn / a.query_blocks) * 8 + (blockIdx.x & 7), tile0 = (turn % a.query_blocks) * MT;
+  __shared__ float4_t sums[CENTRED ? 1 : 2][CENTRED ? 1 : MT][16];  // [..][group of the chunk * 4 + quarter]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, c = lane >> 4;
+  // workgroups of the same rows one after the other on the same chiplet, whose L2 then holds the rows
+  const int shares = (a.query_blocks + a.blocks_each - 1) / a.blocks_each, turn = blockIdx.x >> 3;
+  const int block = (turn / shares) * 8 + (blockIdx.x & 7), query_block0 = (turn % shares) * a.blocks_each;
   if (block >= a.row_blocks) return;
   const int last_tile = (a.num_queries - 1) / kTile, chunks = (a.units + UC - 1) / UC;
-  const long long row0 = (long long)block * (4 * kRowTiles * kTile) + wave * (kRowTiles * kTile), last_row = a.num_rows - 1;
+  const long long row0 = (long long)block * (8 * RT * kTile) + wave * (RT * kTile), last_row = a.num_rows - 1;
 
-  const unsigned char* from[UC];
-  int unit_of[UC];
+  const unsigned char* from[kLoads];
+  int unit_of[kLoads];
 #pragma unroll
-  for (int i = 0; i < UC; ++i) {
+  for (int i = 0; i < kLoads; ++i) {
     const int slot = 4 * i + c;
     unit_of[i] = slot % UC;
-    from[i] = a.codes + min(row0 + slot / UC * kTile + j, last_row) * ((long long)a.units * 16);
+    from[i] = a.codes + min(row0 + j * RT + slot / UC, last_row) * ((long long)a.units * 16);
   }
-  long long groups_of[kRowTiles];
-#pragma unroll
-  for (int t = 0; t < kRowTiles; ++t) groups_of[t] = min(row0 + t * kTile + j, last_row) * a.groups;
-  uint4 words[UC];
-  uint16_t scales[kRowTiles][kGroups], offsets[kRowTiles][kGroups];
+  // (an even quarter has the first row tile's scales and offsets, an odd one the second's; offsets come to the upper half)
+  const uint16_t* groups_of = (CENTRED || c < 2 ? a.scales : a.offsets) + min(row0 + j * RT + (c & 1), last_row) * a.groups;
+  uint4 words[kLoads];
+  Groups<kGroups> held;
   auto load = [&](int chunk) {
 #pragma unroll
-    for (int i = 0; i < UC; ++i) words[i] = *reinterpret_cast<const uint4*>(from[i] + min(chunk * UC + unit_of[i], a.units - 1) * 16);
-#pragma unroll
-    for (int t = 0; t < kRowTiles; ++t)
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const long long at = groups_of[t] + min(chunk * UC / GU + g, a.groups - 1);
-        scales[t][g] = a.scales[at];
-        if (!CENTRED) offsets[t][g] = a.offsets[at];
-      }
+    for (int i = 0; i < kLoads; ++i) words[i] = *reinterpret_cast<const uint4*>(from[i] + min(chunk * UC + unit_of[i], a.units - 1) * 16);
+    held = load_groups<kGroups>(groups_of, chunk * UC / GU, a.groups);
   };
   // piece (u, m, p) of a chunk: 64 x 16 bytes that lie in a row in the planes
-  auto bring = [&](int chunk, int buffer) {
-    for (int piece = wave; piece < kPieces; piece += 4) {
-      const int p = piece % PLANES, m = piece / PLANES % MT, u = piece / PLANES / MT;
-      const _Float16* there = a.planes + p * a.plane + ((size_t)min(tile0 + m, last_tile) * a.padded_units + chunk * UC + u) * (kTile * kUnit) + lane * 8;
+  auto bring = [&](int query_block, int chunk, int buffer) {
+    for (int piece = wave; piece < kPieces; piece += 8) {
+      const int p = piece % PLANES, m = piece / PLANES % MT, u = piece / PLANES / MT, tile = min(query_block * MT + m, last_tile);
+      const _Float16* there = a.planes + p * a.plane + ((size_t)tile * a.padded_units + chunk * UC + u) * (kTile * kUnit) + lane * 8;
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(there)),
                                        (__attribute__((address_space(3))) void*)&queries[buffer][piece][0], 16, 0, 0);
     }
+    if (!CENTRED && wave < MT) {  // the sums of the chunk's groups, a float for each lane
+      const size_t tile = min(query_block * MT + wave, last_tile);
+      const int at = min(chunk * UC / GU * kTile + lane, a.groups * kTile - 1);  // (what is not the chunk's is not looked at)
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(a.sums + tile * a.groups * kTile + at)),
+                                       (__attribute__((address_space(3))) void*)&sums[buffer][wave][0], 4, 0, 0);
+    }
   };
-  float4_t acc[kRowTiles][MT];
-#pragma unroll
-  for (int t = 0; t < kRowTiles; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
-  bring(0, 0);
+  const int query_blocks = min(a.blocks_each, a.query_blocks - query_block0);
+  float4_t acc[RT][MT];
+  int query_block = query_block0, chunk = 0;
+  bring(query_block, 0, 0);
   load(0);
-  for (int chunk = 0; chunk < chunks; ++chunk) {
-    // (what was brought is in LDS once every wavefront has waited for its own loads)
+  for (int step = 0;; ++step) {
+    // What was brought is in LDS once every wavefront has waited for its own loads.  A block's scores are stored behind that wait:
+    // they have the next chunk's work to get there.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    uint32_t word[kRowTiles][UC];
+    const int buffer = step & 1;
+    if (chunk == 0) {
+      if (step > 0) store_scores<RT, MT>(a, acc, (query_block - 1) * MT, c, row0 + j * RT);
+      if (query_block == query_block0 + query_blocks) break;
 #pragma unroll
-    for (int i = 0; i < UC; ++i) {
-      uint32_t slots[4];
-      exchange(words[i], slots);
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) word[(4 * i + q) / UC][(4 * i + q) % UC] = slots[q];
+        for (int m = 0; m < MT; ++m) acc[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    float scale[kRowTiles][kGroups], offset[kRowTiles][kGroups];
+    {
+      uint32_t word[RT][UC];
 #pragma unroll
-    for (int t = 0; t < kRowTiles; ++t)
+      for (int i = 0; i < kLoads; ++i) {
+        uint32_t slots[4];
+        exchange(words[i], slots);
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        scale[t][g] = half_bits(scales[t][g], a.scale_bf16) * 0x1p-14f;
-        // (behind the last group there is nothing)
-        offset[t][g] = CENTRED || chunk * UC / GU + g >= a.groups ? 0.f : half_bits(offsets[t][g], a.scale_bf16);
+        for (int q = 0; q < 4; ++q) word[(4 * i + q) / UC][(4 * i + q) % UC] = slots[q];
       }
-    if (chunk + 1 < chunks) {
-      bring(chunk + 1, (chunk + 1) & 1);
-      load(chunk + 1);
-    }
-    float4_t temp[kRowTiles][MT];
+      Groups<kGroups> quarters[4];
+      from_quarters(held, quarters);
+      float scale[RT][kGroups], offset[RT][kGroups];
 #pragma unroll
-    for (int u = 0; u < UC; ++u) {
-      half8_t query[MT][PLANES];
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int g = 0; g < kGroups; ++g) {
+          scale[t][g] = half_bits(quarters[t][g], a.scale_bf16) * 0x1p-14f;
+          // (behind the last group there is nothing)
+          offset[t][g] = CENTRED || chunk * UC / GU + g >= a.groups ? 0.f : half_bits(quarters[2 + t][g], a.scale_bf16);
+        }
+      if (++chunk == chunks) {
+        chunk = 0;
+        ++query_block;
+      }
+      if (query_block < query_block0 + query_blocks) {
+        bring(query_block, chunk, buffer ^ 1);
+        load(chunk);
+      }
+      float4_t temp[RT][MT];
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) query[m][p] = queries[chunk & 1][(u * MT + m) * PLANES + p][lane];
-      const int group = min(chunk * UC / GU + u / GU, a.groups - 1);
-      float4_t x[MT];
-      if (!CENTRED && (u % GU == GU - 1 || u == UC - 1))
+      for (int u = 0; u < UC; ++u) {
+        half8_t query[MT][PLANES];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          x[m] = *reinterpret_cast<const float4_t*>(a.sums + ((size_t)min(tile0 + m, last_tile) * a.groups + group) * kTile + c * 4);
 #pragma unroll
-      for (int t = 0; t < kRowTiles; ++t) {
-        const half8_t codes = codes_of<CENTRED>(word[t][u]);
+          for (int p = 0; p < PLANES; ++p) query[m][p] = queries[buffer][(u * MT + m) * PLANES + p][lane];
+        float4_t x[MT];
+        if (!CENTRED && (u % GU == GU - 1 || u == UC - 1))
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (u % GU == 0) temp[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
+          for (int m = 0; m < MT; ++m) x[m] = sums[buffer][m][u / GU * 4 + c];
 #pragma unroll
-          for (int p = PLANES - 1; p >= 0; --p) temp[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(query[m][p], codes, temp[t][m], 0, 0, 0);
-          if (u % GU != GU - 1 && u != UC - 1) continue;
+        for (int t = 0; t < RT; ++t) {
+          const half8_t codes = codes_of<CENTRED>(word[t][u]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[t][m][r] = fmaf(scale[t][u / GU], temp[t][m][r], acc[t][m][r]);
-          if (!CENTRED)
+          for (int m = 0; m < MT; ++m) {
+            if (u % GU == 0) temp[t][m] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][m][r] = fmaf(offset[t][u / GU], x[m][r], acc[t][m][r]);
+            for (int p = PLANES - 1; p >= 0; --p) temp[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(query[m][p], codes, temp[t][m], 0, 0, 0);
+          }
         }
+        if (u % GU != GU - 1 && u != UC - 1) continue;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[t][m][r] = fmaf(scale[t][u / GU], temp[t][m][r], acc[t][m][r]);
+              if (!CENTRED) acc[t][m][r] = fmaf(offset[t][u / GU], x[m][r], acc[t][m][r]);
+            }
       }
     }
   }
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int query = (tile0 + m) * kTile + c * 4 + r;
-      if (query >= a.num_queries) continue;
-      const int exponent = a.exponents[query];
-#pragma unroll
-      for (int t = 0; t < kRowTiles; ++t)
-        if (row0 + t * kTile + j <= last_row) store_score(a, query, row0 + t * kTile + j, acc[t][m][r], exponent);
-    }
 }
 
 inline int units_of(int num_dims) { return (num_dims + kUnit - 1) / kUnit; }
@@ -488,6 +578,7 @@ struct ScoresPlan {
   int query_tiles;                          // of a workgroup; 0: few queries
   bool own;                                 // few queries, laid out by the workgroups themselves
   int split, waves, query_blocks, row_blocks;
+  int blocks_each;                          // many queries: blocks of them that a workgroup goes over
   size_t lds;
   ScoresPlan(long long num_rows, int num_dims, int group, int query_type, int num_queries) {
     const int units = units_of(num_dims), tiles = (num_queries + kTile - 1) / kTile;
@@ -498,11 +589,14 @@ struct ScoresPlan {
     query_tiles = tiles > 1 && blocks * query_blocks >= 256 ? (tiles + query_blocks - 1) / query_blocks : 0;
     own = false;
     lds = 0;
+    blocks_each = 1;
     if (query_tiles) {
       chunk = units <= 2 ? 2 : 4;
       split = 1;
-      waves = 4;
+      waves = 8;
       row_blocks = (int)blocks;
+      // (as few workgroups as keep the machine full: each begins with loads that nothing hides)
+      blocks_each = (int)std::max<long long>(1, std::min<long long>(query_blocks, blocks * query_blocks / 1024));
     } else {
       chunk = std::min(units, 4);
       query_blocks = tiles;
@@ -556,10 +650,10 @@ void launch_few_of(const ScoresArgs& a, const ScoresPlan& p, int query_type, hip
 
 template <int UC, int GU, int MT, int PLANES>
 void launch_many(const ScoresArgs& a, hipStream_t stream) {
-  const long long grid = ((long long)a.row_blocks + 7) / 8 * 8 * a.query_blocks;
+  const long long grid = ((long long)a.row_blocks + 7) / 8 * 8 * ((a.query_blocks + a.blocks_each - 1) / a.blocks_each);
   want(grid <= 0x7fffffff, "scores: too many rows and queries");
-  if (a.offsets) hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  if (a.offsets) hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, false>), dim3((unsigned)grid), dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, true>), dim3((unsigned)grid), dim3(512), 0, stream, a);
 }
 template <int UC, int GU, int MT>
 void launch_many_of(const ScoresArgs& a, const ScoresPlan& p, hipStream_t stream) {
@@ -643,6 +737,7 @@ int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offs
     a.query_blocks = p.query_blocks;
     a.row_blocks = p.row_blocks;
     a.split = p.split;
+    a.blocks_each = p.blocks_each;
     const ScoresScratch w(workspace, num_queries, p);
     want(w.bytes == 0 || (workspace && workspace_bytes >= (long long)w.bytes), "scores: the workspace is too small");
     a.planes = w.planes;
