@@ -86,6 +86,7 @@ void launch_pack(const PackArgs& a, hipStream_t stream) {
 // Queries are laid out as the lanes want them: for a tile of 16 queries and a unit of 32 elements, 16 bytes for every quarter of the
 // unit and query.  That is a launch of its own (prepare_kernel), or, where they are few and short, every workgroup's first
 // step, into its LDS.
+constexpr int kManyWaves = 4, kManyResident = 768;  // wavefronts of a workgroup for many queries, and such workgroups that the machine holds
 constexpr int kTile = 16, kUnit = 32, kRowTiles = 4;  // queries or rows of a matrix product, elements of it; row tiles of a wavefront
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -109,7 +110,7 @@ struct ScoresArgs {
   int padded_units;        // units that the planes hold: the last are zero
   _Float16* planes;        // [planes][query tile][unit][quarter][16][8]
   size_t plane;            // elements of one plane
-  int* exponents;          // of every query: what its scores are to be scaled by
+  signed char* exponents;  // of every query: what its scores are to be scaled by
   float* sums;             // [query tile][group][16]: sums of the groups' elements
   int query_blocks, row_blocks, split, blocks_each;
 };
@@ -130,7 +131,7 @@ __device__ inline int exponent_of(const T* q, int num_dims, float* per_wave) {
   __syncthreads();
   for (int w = 0; w < threads / 64; ++w) most = fmaxf(most, per_wave[w]);
   __syncthreads();
-  return most > 0.f && most < INFINITY ? ilogbf(most) : 14;
+  return most > 0.f && most < INFINITY ? max(ilogbf(most), -126) : 14;  // (a byte holds it)
 }
 // Eight elements, a quarter of a unit, in the order in which the codes of a word come apart: 0 4 1 5 2 6 3 7.
 template <typename T>
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(ScoresArgs a, int planes) 
   const bool there = m < a.num_queries;  // (the last tile is filled up with zeros)
   const T* q = static_cast<const T*>(a.queries) + (there ? m : 0) * a.query_stride;
   const int num_dims = there ? a.num_dims : 0, exponent = exponent_of(q, num_dims, per_wave);
-  if (tid == 0) a.exponents[m] = exponent;
+  if (tid == 0) a.exponents[m] = (signed char)exponent;
   _Float16* to = a.planes + (size_t)tile * kTile * a.padded_units * kUnit;
   for (int w = tid; w < a.padded_units * 4; w += 256) {
     half8_t high, low;
@@ -252,50 +253,91 @@ __device__ inline void exchange(uint4 words, uint32_t (&slots)[4]) {
   slots[3] = hi[1];
 }
 
-// A lane's scores: RT rows one after the other from `row` on, for four queries of every tile.
+// Among four neighbouring lanes: of lane l, x[0..3] are row 0..3 of its column; afterwards they are column 0..3 of row l.
+__device__ inline void transpose_quad(uint32_t (&x)[4]) {
+  const int l = threadIdx.x & 3;
+  auto swap = [&](uint32_t& low, uint32_t& high, bool upper, auto dpp) {
+    const uint32_t mine = upper ? low : high, theirs = dpp(mine);
+    low = upper ? theirs : low;
+    high = upper ? high : theirs;
+  };
+  auto next = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true); };     // lanes 1 0 3 2
+  auto over = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true); };     // lanes 2 3 0 1
+  swap(x[0], x[1], l & 1, next);
+  swap(x[2], x[3], l & 1, next);
+  swap(x[0], x[2], l & 2, over);
+  swap(x[1], x[3], l & 2, over);
+}
+
+// A lane's scores: RT rows one after the other from `row` on, for four queries of every tile, whose exponents are the bytes of
+// a word.  Where a score is two bytes four neighbouring lanes exchange theirs first: each then has all of their rows for one of
+// the four queries, and stores 16 bytes at a time.
 template <int RT, int MT>
-__device__ inline void store_scores(const ScoresArgs& a, const float4_t (&acc)[RT][MT], int tile0, int c, long long row, const int* exponents = nullptr) {
-  const int rows = (int)min((long long)RT, a.num_rows - row);
-  float bias[RT];
+__device__ inline void store_scores(const ScoresArgs& a, const float4_t (&acc)[RT][MT], int tile0, int c, long long row, const uint32_t (&exponents)[MT],
+                                    const float (&bias)[RT]) {
+  const int l = threadIdx.x & 3;
+  const long long first = row - l * RT;  // of the four lanes' rows
 #pragma unroll
-  for (int t = 0; t < RT; ++t) bias[t] = a.bias && t < rows ? a.bias[row + t] : 0.f;
+  for (int m = 0; m < MT; ++m) {
+    auto score = [&](int r, int t) { return a.alpha * ldexpf(acc[t][m][r], (signed char)(exponents[m] >> (8 * r))) + bias[t]; };
+    if (a.out_type == TYPE_F32) {
+      const int rows = (int)max(0ll, min((long long)RT, a.num_rows - row));
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int query = (tile0 + m) * kTile + c * 4 + r;
-      if (query < a.num_queries && rows > 0) {
-        const int exponent = exponents ? exponents[c * 4 + r] : a.exponents[query];
-        const long long at = query * a.out_stride + row;
+      for (int r = 0; r < 4; ++r) {
+        const int query = (tile0 + m) * kTile + c * 4 + r;
         LoosePack<float, RT> y;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) y.at[t] = a.alpha * ldexpf(acc[t][m][r], exponent) + bias[t];
-        if (a.out_type == TYPE_F32) {
-          float* to = static_cast<float*>(a.out) + at;
-          if (rows == RT) *reinterpret_cast<LoosePack<float, RT>*>(to) = y;
-          else
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-              if (t < rows) to[t] = y.at[t];
-        } else {
-          uint16_t* to = static_cast<uint16_t*>(a.out) + at;
-          uint32_t words[RT / 2];
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            const uint16_t bits = a.out_type == TYPE_BF16 ? narrow<bf16>(y.at[t]).bits : __builtin_bit_cast(uint16_t, (_Float16)y.at[t]);
-            words[t / 2] = t % 2 ? words[t / 2] | (uint32_t)bits << 16 : bits;
-          }
+        for (int t = 0; t < RT; ++t) y.at[t] = score(r, t);
+        float* to = static_cast<float*>(a.out) + query * a.out_stride + row;
+        if (query < a.num_queries) {
           if (rows == RT) {
-            if constexpr (RT == 2) *reinterpret_cast<loose32*>(to) = words[0];
-            else *reinterpret_cast<loose64*>(to) = (uint64_t)words[RT / 2 - 1] << 32 | words[0];
+            *reinterpret_cast<LoosePack<float, RT>*>(to) = y;
           } else {
 #pragma unroll
             for (int t = 0; t < RT; ++t)
-              if (t < rows) to[t] = (uint16_t)(words[t / 2] >> (t % 2 * 16));
+              if (t < rows) to[t] = y.at[t];
           }
         }
       }
+    } else {
+      const int query = (tile0 + m) * kTile + c * 4 + l, rows = (int)max(0ll, min(4ll * RT, a.num_rows - first));
+      const bool there = query < a.num_queries && rows > 0;
+      uint32_t words[RT / 2][4];  // two rows in a word
+#pragma unroll
+      for (int w = 0; w < RT / 2; ++w) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float low = score(r, 2 * w), high = score(r, 2 * w + 1);
+          words[w][r] = a.out_type == TYPE_BF16 ? narrow<bf16>(low).bits | (uint32_t)narrow<bf16>(high).bits << 16
+                                                : __builtin_bit_cast(uint16_t, (_Float16)low) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)high) << 16;
+        }
+        transpose_quad(words[w]);
+      }
+      uint16_t* to = static_cast<uint16_t*>(a.out) + query * a.out_stride + first;
+      if (there && rows == 4 * RT) {
+#pragma unroll
+        for (int i = 0; i < RT / 2; ++i) {
+          struct __attribute__((packed, aligned(2))) Loose128 {
+            uint32_t at[4];
+          } eight;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) eight.at[e] = words[(i * 4 + e) % (RT / 2)][(i * 4 + e) / (RT / 2)];
+          *reinterpret_cast<Loose128*>(to + i * 8) = eight;
+        }
+      } else if (there) {
+#pragma unroll
+        for (int i = 0; i < 4 * RT; ++i)
+          if (i < rows) to[i] = (uint16_t)(words[i / 2 % (RT / 2)][i / 2 / (RT / 2)] >> (i % 2 * 16));
+      }
     }
+  }
+}
+// the exponents of queries c * 4 to c * 4 + 3 of a tile
+__device__ inline uint32_t exponents_at(const signed char* of_tile, int c) { return *reinterpret_cast<const uint32_t*>(of_tile + c * 4); }
+template <int RT>
+__device__ inline void bias_at(const ScoresArgs& a, long long row, float (&bias)[RT]) {
+#pragma unroll
+  for (int t = 0; t < RT; ++t) bias[t] = a.bias && row + t < a.num_rows ? a.bias[row + t] : 0.f;
 }
 
 // Few queries: bound by the rows' codes.  A wavefront has 64 rows (four tiles of 16) and one tile of queries, and goes over the
@@ -352,14 +394,14 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
   const int own_queries = min(kTile, a.num_queries), own_plane = a.padded_units * kUnit * own_queries;
   _Float16* own = reinterpret_cast<_Float16*>(lds);
   float* own_sums = reinterpret_cast<float*>(own + (size_t)PLANES * own_plane);
-  int* own_exponents = reinterpret_cast<int*>(own_sums + (CENTRED ? 0 : kTile * a.groups));
+  signed char* own_exponents = reinterpret_cast<signed char*>(own_sums + (CENTRED ? 0 : kTile * a.groups));
   float* per_wave = reinterpret_cast<float*>(own_exponents + kTile);
   float4_t* partial = reinterpret_cast<float4_t*>(OWN ? reinterpret_cast<unsigned char*>(per_wave + 8) : lds);
   if (OWN) {
     for (int i = 0; i < own_queries; ++i) {
       const T* q = static_cast<const T*>(a.queries) + i * a.query_stride;
       const int exponent = exponent_of(q, a.num_dims, per_wave);
-      if (threadIdx.x == 0) own_exponents[i] = exponent;
+      if (threadIdx.x == 0) own_exponents[i] = (signed char)exponent;
       for (int w = threadIdx.x; w < a.padded_units * 4; w += blockDim.x) {
         half8_t high, low;
         planes_of_eight(q, w * 8, a.num_dims, exponent, high, low);
@@ -431,16 +473,19 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
 #pragma unroll
       for (int t = 0; t < kRowTiles; ++t) acc[t][0] += partial[((s * per_block + in_block) * kRowTiles + t) * 64 + lane];
   }
-  store_scores<kRowTiles, 1>(a, acc, tile, c, row0 + j * kRowTiles, OWN ? own_exponents : nullptr);
+  const uint32_t exponents[1] = {exponents_at(OWN ? own_exponents : a.exponents + tile * kTile, c)};
+  float bias[kRowTiles];
+  bias_at(a, row0 + j * kRowTiles, bias);
+  store_scores<kRowTiles, 1>(a, acc, tile, c, row0 + j * kRowTiles, exponents, bias);
 }
 
-// Many queries: a workgroup of eight wavefronts has 256 rows, 32 for each wavefront, and goes over `blocks_each` blocks of MT
+// Many queries: a workgroup of kManyWaves wavefronts has 32 rows for each of them, and goes over `blocks_each` blocks of MT
 // tiles of queries, chunk by chunk of UC units.  The queries' planes of a chunk go through LDS (straight from memory, the
-// next chunk's while this one is at work), so eight wavefronts share what they read of them; a unit's planes stay in
+// next chunk's while this one is at work), so the wavefronts share what they read of them; a unit's planes stay in
 // registers over the wavefront's two row tiles.  Rows 2 j and 2 j + 1 are lane j's in the two tiles, so that it stores them
 // together.
 template <int UC, int GU, int MT, int PLANES, bool CENTRED>
-__global__ void __launch_bounds__(512, 4) scores_many_kernel(ScoresArgs a) {
+__global__ void __launch_bounds__(64 * kManyWaves, 3) scores_many_kernel(ScoresArgs a) {
   constexpr int RT = 2, kLoads = UC * RT / 4;
   constexpr int kGroups = (UC + GU - 1) / GU, kPieces = UC * MT * PLANES;  // pieces of 1 KB: what a wavefront reads at once
   __shared__ half8_t queries[2][kPieces][64];
@@ -451,7 +496,7 @@ __global__ void __launch_bounds__(512, 4) scores_many_kernel(ScoresArgs a) {
   const int block = (turn / shares) * 8 + (blockIdx.x & 7), query_block0 = (turn % shares) * a.blocks_each;
   if (block >= a.row_blocks) return;
   const int last_tile = (a.num_queries - 1) / kTile, chunks = (a.units + UC - 1) / UC;
-  const long long row0 = (long long)block * (8 * RT * kTile) + wave * (RT * kTile), last_row = a.num_rows - 1;
+  const long long row0 = (long long)block * (kManyWaves * RT * kTile) + wave * (RT * kTile), last_row = a.num_rows - 1;
 
   const unsigned char* from[kLoads];
   int unit_of[kLoads];
@@ -472,7 +517,7 @@ __global__ void __launch_bounds__(512, 4) scores_many_kernel(ScoresArgs a) {
   };
   // piece (u, m, p) of a chunk: 64 x 16 bytes that lie in a row in the planes
   auto bring = [&](int query_block, int chunk, int buffer) {
-    for (int piece = wave; piece < kPieces; piece += 8) {
+    for (int piece = wave; piece < kPieces; piece += kManyWaves) {
       const int p = piece % PLANES, m = piece / PLANES % MT, u = piece / PLANES / MT, tile = min(query_block * MT + m, last_tile);
       const _Float16* there = a.planes + p * a.plane + ((size_t)tile * a.padded_units + chunk * UC + u) * (kTile * kUnit) + lane * 8;
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(there)),
@@ -487,6 +532,9 @@ __global__ void __launch_bounds__(512, 4) scores_many_kernel(ScoresArgs a) {
   };
   const int query_blocks = min(a.blocks_each, a.query_blocks - query_block0);
   float4_t acc[RT][MT];
+  uint32_t exponents[MT];
+  float bias[RT];
+  bias_at(a, row0 + j * RT, bias);
   int query_block = query_block0, chunk = 0;
   bring(query_block, 0, 0);
   load(0);
@@ -497,8 +545,10 @@ __global__ void __launch_bounds__(512, 4) scores_many_kernel(ScoresArgs a) {
     __syncthreads();
     const int buffer = step & 1;
     if (chunk == 0) {
-      if (step > 0) store_scores<RT, MT>(a, acc, (query_block - 1) * MT, c, row0 + j * RT);
+      if (step > 0) store_scores<RT, MT>(a, acc, (query_block - 1) * MT, c, row0 + j * RT, exponents, bias);
       if (query_block == query_block0 + query_blocks) break;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) exponents[m] = exponents_at(a.exponents + min(query_block * MT + m, last_tile) * kTile, c);
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -585,7 +635,7 @@ struct ScoresPlan {
     planes = planes_of(query_type);
     groups = (num_dims + group - 1) / group;
     query_blocks = (tiles + 3) / 4;
-    const long long blocks = (num_rows + 255) / 256;
+    const long long blocks = (num_rows + kManyWaves * 32 - 1) / (kManyWaves * 32);
     query_tiles = tiles > 1 && blocks * query_blocks >= 256 ? (tiles + query_blocks - 1) / query_blocks : 0;
     own = false;
     lds = 0;
@@ -593,10 +643,17 @@ struct ScoresPlan {
     if (query_tiles) {
       chunk = units <= 2 ? 2 : 4;
       split = 1;
-      waves = 8;
+      waves = kManyWaves;
       row_blocks = (int)blocks;
-      // (as few workgroups as keep the machine full: each begins with loads that nothing hides)
-      blocks_each = (int)std::max<long long>(1, std::min<long long>(query_blocks, blocks * query_blocks / 1024));
+      // into how many workgroups the query blocks of the same rows are divided: rounds of workgroups times the chunks of each,
+      // and the loads that nothing hides at its beginning
+      const int chunks = (units + chunk - 1) / chunk;
+      long long least = 0;
+      for (int shares = 1; shares <= std::min(query_blocks, 16); ++shares) {
+        const int each = (query_blocks + shares - 1) / shares;
+        const long long time = (blocks * ((query_blocks + each - 1) / each) + kManyResident - 1) / kManyResident * ((long long)each * chunks + 2);
+        if (shares == 1 || time < least) least = time, blocks_each = each;
+      }
     } else {
       chunk = std::min(units, 4);
       query_blocks = tiles;
@@ -609,7 +666,7 @@ struct ScoresPlan {
     }
     padded_units = (units + chunk - 1) / chunk * chunk;
     if (!query_tiles) {
-      const size_t laid_out = (size_t)padded_units * kUnit * std::min(num_queries, kTile) * planes * 2 + (size_t)groups * kTile * 4 + kTile * 4 + 32;
+      const size_t laid_out = (size_t)padded_units * kUnit * std::min(num_queries, kTile) * planes * 2 + (size_t)groups * kTile * 4 + kTile + 32;
       own = tiles == 1 && laid_out <= 32768;
       lds = (own ? (laid_out + 15) / 16 * 16 : 0) + (size_t)(split > 1 ? (split - 1) * (waves / split) : 0) * kRowTiles * 64 * sizeof(float4_t);
     }
@@ -618,7 +675,7 @@ struct ScoresPlan {
 
 struct ScoresScratch {
   _Float16* planes;
-  int* exponents;
+  signed char* exponents;
   float* sums;
   size_t plane, bytes;
   ScoresScratch(void* memory, int num_queries, const ScoresPlan& p) {
@@ -626,7 +683,7 @@ struct ScoresScratch {
     const size_t queries = p.own ? 0 : (size_t)(num_queries + kTile - 1) / kTile * kTile;
     plane = queries * p.padded_units * kUnit;
     planes = s.part<_Float16>(plane * p.planes);
-    exponents = s.part<int>(queries);
+    exponents = s.part<signed char>(queries);
     sums = s.part<float>(queries * p.groups);
     bytes = s.used();
   }
@@ -652,8 +709,8 @@ template <int UC, int GU, int MT, int PLANES>
 void launch_many(const ScoresArgs& a, hipStream_t stream) {
   const long long grid = ((long long)a.row_blocks + 7) / 8 * 8 * ((a.query_blocks + a.blocks_each - 1) / a.blocks_each);
   want(grid <= 0x7fffffff, "scores: too many rows and queries");
-  if (a.offsets) hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, false>), dim3((unsigned)grid), dim3(512), 0, stream, a);
-  else hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, true>), dim3((unsigned)grid), dim3(512), 0, stream, a);
+  if (a.offsets) hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, false>), dim3((unsigned)grid), dim3(64 * kManyWaves), 0, stream, a);
+  else hipLaunchKernelGGL((scores_many_kernel<UC, GU, MT, PLANES, true>), dim3((unsigned)grid), dim3(64 * kManyWaves), 0, stream, a);
 }
 template <int UC, int GU, int MT>
 void launch_many_of(const ScoresArgs& a, const ScoresPlan& p, hipStream_t stream) {
