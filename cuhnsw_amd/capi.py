@@ -23,6 +23,7 @@ SYMBOLS = [
     "cuhnsw_get_items", "cuhnsw_search_items", "cuhnsw_get_labels", "cuhnsw_pack_items", "cuhnsw_lookup_rows",
     "cuhnsw_lookup_grad_workspace", "cuhnsw_lookup_rows_grad", "cuhnsw_pack_rows", "cuhnsw_packed_scores_workspace",
     "cuhnsw_packed_scores", "cuhnsw_select_beams_workspace", "cuhnsw_select_beams", "cuhnsw_reorder_states",
+    "cuhnsw_use_device",
 ]
 
 _lib = None
@@ -75,6 +76,7 @@ def load():
   l.cuhnsw_search_items.argtypes = [vp, vp, ci, cf, ci, ci, vp, vp, vp]
   l.cuhnsw_get_labels.argtypes = [vp, vp]
   l.cuhnsw_pack_items.argtypes = [vp, ci, vp, vp, vp, ci, vp]
+  l.cuhnsw_use_device.argtypes = [ci, ctypes.POINTER(ci)]
   l.cuhnsw_lookup_rows.argtypes = [vp, ci, ll, ll, ci, vp, ci, ll, cf, vp, ci, vp]
   l.cuhnsw_lookup_grad_workspace.argtypes = [ll, ll, ci]
   l.cuhnsw_lookup_grad_workspace.restype = ll

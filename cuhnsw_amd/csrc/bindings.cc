@@ -173,32 +173,45 @@ static void CopyBytes(py::array dst, py::array src) {
 static void CheckCall(int rc) {
   if (rc != 0) throw std::runtime_error(cuhnsw_last_error(nullptr));
 }
+struct OnDevice {  // the launches' device is the current one meanwhile
+  int before = -1;
+  explicit OnDevice(int device) { CheckCall(cuhnsw_use_device(device, &before)); }
+  ~OnDevice() {
+    int there;
+    (void)cuhnsw_use_device(before, &there);
+  }
+};
 static void LookupRows(uintptr_t table, int table_type, long long num_rows, long long row_stride, int num_dims, uintptr_t ids, int ids_64,
-                       long long num_ids, float scale, uintptr_t out, int out_type, uintptr_t stream) {
+                       long long num_ids, float scale, uintptr_t out, int out_type, int device, uintptr_t stream) {
+  const OnDevice on(device);
   CheckCall(cuhnsw_lookup_rows((void*)table, table_type, num_rows, row_stride, num_dims, (void*)ids, ids_64, num_ids, scale, (void*)out,
                                out_type, (void*)stream));
 }
 static void LookupRowsGrad(uintptr_t grad, int grad_type, long long grad_stride, uintptr_t ids, int ids_64, long long num_ids,
                            long long num_rows, int num_dims, float scale, uintptr_t out, int out_type, uintptr_t workspace,
-                           long long workspace_bytes, uintptr_t stream) {
+                           long long workspace_bytes, int device, uintptr_t stream) {
+  const OnDevice on(device);
   CheckCall(cuhnsw_lookup_rows_grad((void*)grad, grad_type, grad_stride, (void*)ids, ids_64, num_ids, num_rows, num_dims, scale, (void*)out,
                                     out_type, (void*)workspace, workspace_bytes, (void*)stream));
 }
 static void PackRows(uintptr_t rows, int type, long long row_stride, long long num_rows, int num_dims, int group, uintptr_t codes,
-                     uintptr_t scales, uintptr_t offsets, int scale_type, uintptr_t stream) {
+                     uintptr_t scales, uintptr_t offsets, int scale_type, int device, uintptr_t stream) {
+  const OnDevice on(device);
   CheckCall(cuhnsw_pack_rows((void*)rows, type, row_stride, num_rows, num_dims, group, (void*)codes, (void*)scales, (void*)offsets, scale_type,
                              (void*)stream));
 }
 static void PackedScores(uintptr_t codes, uintptr_t scales, uintptr_t offsets, int scale_type, long long num_rows, int num_dims, int group,
                          uintptr_t queries, int query_type, long long query_stride, int num_queries, float alpha, uintptr_t bias,
-                         uintptr_t out, int out_type, long long out_stride, uintptr_t workspace, long long workspace_bytes, uintptr_t stream) {
+                         uintptr_t out, int out_type, long long out_stride, uintptr_t workspace, long long workspace_bytes, int device, uintptr_t stream) {
+  const OnDevice on(device);
   CheckCall(cuhnsw_packed_scores((void*)codes, (void*)scales, (void*)offsets, scale_type, num_rows, num_dims, group, (void*)queries, query_type,
                                  query_stride, num_queries, alpha, (const float*)bias, (void*)out, out_type, out_stride, (void*)workspace,
                                  workspace_bytes, (void*)stream));
 }
 static void SelectBeams(uintptr_t scores, int type, long long stride_b, long long stride_k, int num_batch, int num_beams, int num_values,
                         uintptr_t beams, uintptr_t finished, int end, int normalise, int num, uintptr_t totals, uintptr_t parents,
-                        uintptr_t tokens, uintptr_t workspace, long long workspace_bytes, uintptr_t stream) {
+                        uintptr_t tokens, uintptr_t workspace, long long workspace_bytes, int device, uintptr_t stream) {
+  const OnDevice on(device);
   CheckCall(cuhnsw_select_beams((void*)scores, type, stride_b, stride_k, num_batch, num_beams, num_values, (const float*)beams,
                                 (const unsigned char*)finished, end, normalise, num, (float*)totals, (int*)parents, (int*)tokens,
                                 (void*)workspace, workspace_bytes, (void*)stream));
@@ -206,7 +219,8 @@ static void SelectBeams(uintptr_t scores, int type, long long stride_b, long lon
 static void ReorderStates(const std::vector<uintptr_t>& from, const std::vector<uintptr_t>& to, const std::vector<long long>& stride_b,
                           const std::vector<long long>& stride_k, const std::vector<long long>& bytes, uintptr_t parents,
                           long long parent_stride_b, long long parent_stride_k, int num_batch, int num_beams, int num_picked,
-                          uintptr_t stream) {
+                          int device, uintptr_t stream) {
+  const OnDevice on(device);
   const size_t n = from.size();
   if (to.size() != n || stride_b.size() != n || stride_k.size() != n || bytes.size() != n) throw std::runtime_error("reorder: lists of one length are wanted");
   CheckCall(cuhnsw_reorder_states(reinterpret_cast<const void* const*>(from.data()), reinterpret_cast<void* const*>(to.data()), stride_b.data(),

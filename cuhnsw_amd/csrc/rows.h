@@ -58,9 +58,13 @@ void set_call_error(const char* message) noexcept;
 template <typename F>
 int call_guarded(F&& f) noexcept {
   try {
-    int devices = 0;
-    if (hipGetDeviceCount(&devices) != hipSuccess || devices == 0) {
+    static const bool any_device = [] {
+      int devices = 0;
+      const bool there = hipGetDeviceCount(&devices) == hipSuccess && devices > 0;
       (void)hipGetLastError();
+      return there;
+    }();
+    if (!any_device) {
       set_call_error("no HIP device available: this call needs a GPU");
       return -1;
     }

@@ -425,6 +425,17 @@ using namespace cuhnsw_amd;
 
 extern "C" {
 
+int cuhnsw_use_device(int device, int* before) {
+  int now = -1;
+  if (!before || hipGetDevice(&now) != hipSuccess || (now != device && hipSetDevice(device) != hipSuccess)) {
+    (void)hipGetLastError();
+    set_call_error("no such HIP device");
+    return -1;
+  }
+  *before = now;
+  return 0;
+}
+
 int cuhnsw_lookup_rows(const void* table, int table_type, long long num_rows, long long row_stride, int num_dims, const void* ids,
                        int ids_64, long long num_ids, float scale, void* out, int out_type, void* stream) {
   return call_guarded([&] {

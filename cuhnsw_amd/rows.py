@@ -53,27 +53,29 @@ def _rows(x, name):
 
 
 def _same_device(first, *others):
-  _check(first.is_cuda, "the tensors have to be on the GPU")
+  """The number of the GPU that all of the tensors are on."""
+  device = first.get_device()
+  _check(device >= 0, "the tensors have to be on the GPU")
   for x in others:
-    _check(x is None or x.device == first.device, "the tensors are on different devices")
+    _check(x is None or x.get_device() == device, "the tensors are on different devices")
+  return device
 
 
 def _number(x, name):
-  if not isinstance(x, numbers.Real) or isinstance(x, bool):
-    raise TypeError("%s is a number, not %s" % (name, type(x).__name__))
-  return float(x)
+  if type(x) is not float:
+    if not isinstance(x, numbers.Real) or isinstance(x, bool):
+      raise TypeError("%s is a number, not %s" % (name, type(x).__name__))
+    x = float(x)
+  return x
 
 
-def _stream(device):
-  return torch.cuda.current_stream(device).cuda_stream
+# (the native calls take the device's number and make it the current one while they launch; the handle of torch's current
+# stream is asked for without the object around it where that is possible: together a few microseconds a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _on(device):
-  return torch.cuda.device(device)
-
-
-def _workspace(size, device):
-  return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+def _workspace(size, like):
+  return like.new_empty(size, dtype=torch.uint8) if size else None
 
 
 def _address(x):
@@ -84,31 +86,58 @@ def _address(x):
 _IDS = {torch.int32: 0, torch.int64: 1}
 
 
-def _lookup(table, ids, scale, dtype):
-  stride = _rows(table, "table")
-  flat = ids.reshape(-1)
-  out = torch.empty(flat.shape[0], table.shape[1], dtype=dtype, device=table.device)
-  if flat.stride(0) != 1:
-    flat = flat.contiguous()
-  with _on(table.device):
-    _native.lookup_rows(table.data_ptr(), _TYPES[table.dtype], table.shape[0], stride, table.shape[1], flat.data_ptr(), _IDS[ids.dtype],
-                        flat.shape[0], scale, out.data_ptr(), _TYPES[dtype], _stream(table.device))
-  return out.view(*ids.shape, table.shape[1])
+def _flat(ids):
+  ids = ids if ids.dim() == 1 else ids.reshape(-1)
+  return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def _lookup(table, flat, scale, dtype, device):
+  dims = table.shape[1]
+  out = table.new_empty((flat.shape[0], dims), dtype=dtype)
+  _native.lookup_rows(table.data_ptr(), _TYPES[table.dtype], table.shape[0], _rows(table, "table"), dims, flat.data_ptr(), _IDS[flat.dtype],
+                      flat.shape[0], scale, out.data_ptr(), _TYPES[dtype], device, _raw_stream(device))
+  return out
+
+
+def _grad_workspace(flat, num_rows, dims):
+  return _native.lookup_grad_workspace(flat.shape[0], num_rows, dims)
+
+
+def _lookup_grad(grad, flat, num_rows, dims, scale, dtype, size, device):
+  stride = dims
+  if not grad.is_contiguous():
+    grad = grad.reshape(-1, dims)
+    if dims > 1 and grad.stride(1) != 1:
+      grad = grad.contiguous()
+    stride = _rows(grad, "grad")
+  out = grad.new_empty((num_rows, dims), dtype=dtype)
+  work = grad.new_empty(size, dtype=torch.uint8) if size else None
+  _native.lookup_rows_grad(grad.data_ptr(), _TYPES[grad.dtype], stride, flat.data_ptr(), _IDS[flat.dtype], flat.shape[0], num_rows, dims, scale,
+                           out.data_ptr(), _TYPES[dtype], work.data_ptr() if size else 0, size, device, _raw_stream(device))
+  return out
 
 
 class _Lookup(torch.autograd.Function):
+  """(What can be found out in the forward pass is: the backward pass runs on autograd's own thread, where Python is slow.)"""
 
   @staticmethod
-  def forward(ctx, table, ids, scale, dtype):
-    ctx.save_for_backward(ids)
-    ctx.scale, ctx.num_rows, ctx.dtype = scale, table.shape[0], table.dtype
-    return _lookup(table, ids, scale, dtype)
+  def forward(ctx, table, flat, shape, scale, dtype, device):
+    num_rows, dims = table.shape
+    ctx.save_for_backward(flat)
+    ctx.rest = num_rows, dims, scale, table.dtype, _grad_workspace(flat, num_rows, dims), device
+    out = _lookup(table, flat, scale, dtype, device)
+    return out if shape is None else out.view(shape)
+
+  @staticmethod
+  def backward(ctx, grad):
+    if torch.is_grad_enabled():  # (a graph of the gradient is wanted: one that says that it cannot be had)
+      return _Lookup.backward_of_once(ctx, grad)
+    return _lookup_grad(grad, *ctx.saved_tensors, *ctx.rest), None, None, None, None, None
 
   @staticmethod
   @torch.autograd.function.once_differentiable
-  def backward(ctx, grad):
-    ids, = ctx.saved_tensors
-    return lookup_grad(grad, ids, ctx.num_rows, ctx.scale, ctx.dtype), None, None, None
+  def backward_of_once(ctx, grad):
+    return _lookup_grad(grad, *ctx.saved_tensors, *ctx.rest), None, None, None, None, None
 
 
 def lookup(table, ids, scale=1.0, dtype=None):
@@ -121,12 +150,15 @@ def lookup(table, ids, scale=1.0, dtype=None):
   _tensor(ids, "ids", types=_IDS)
   scale = _number(scale, "scale")
   dtype = dtype or table.dtype
-  _check(dtype in (table.dtype, torch.float32), "the result has the table's type or is float32")
+  _check(dtype is table.dtype or dtype is torch.float32, "the result has the table's type or is float32")
   _check(table.shape[1] > 0, "the table's rows are empty")
-  _same_device(table, ids)
+  _rows(table, "table")
+  device = _same_device(table, ids)
+  flat, shape = _flat(ids), None if ids.dim() == 1 else (*ids.shape, table.shape[1])
   if table.requires_grad and torch.is_grad_enabled():
-    return _Lookup.apply(table, ids, scale, dtype)
-  return _lookup(table, ids, scale, dtype)
+    return _Lookup.apply(table, flat, shape, scale, dtype, device)
+  out = _lookup(table, flat, scale, dtype, device)
+  return out if shape is None else out.view(shape)
 
 
 def lookup_grad(grad, ids, num_rows, scale=1.0, dtype=None):
@@ -143,18 +175,8 @@ def lookup_grad(grad, ids, num_rows, scale=1.0, dtype=None):
   _check(grad.dim() == ids.dim() + 1 and grad.shape[:-1] == ids.shape, "grad has the shape [*ids.shape, dims]")
   _check(grad.shape[-1] > 0, "the rows of grad are empty")
   _check(isinstance(num_rows, int) and num_rows >= 0, "num_rows is a whole number that is not negative")
-  _same_device(grad, ids)
-  dims, flat = grad.shape[-1], ids.reshape(-1).contiguous()
-  grad = grad.reshape(-1, dims)
-  if dims > 1 and grad.stride(1) != 1:
-    grad = grad.contiguous()
-  out = torch.empty(num_rows, dims, dtype=dtype, device=grad.device)
-  with _on(grad.device):
-    size = _native.lookup_grad_workspace(flat.shape[0], num_rows, dims)
-    work = _workspace(size, grad.device)
-    _native.lookup_rows_grad(grad.data_ptr(), _TYPES[grad.dtype], _rows(grad, "grad"), flat.data_ptr(), _IDS[ids.dtype], flat.shape[0],
-                             num_rows, dims, scale, out.data_ptr(), _TYPES[dtype], _address(work), size, _stream(grad.device))
-  return out
+  device, flat, dims = _same_device(grad, ids), _flat(ids), grad.shape[-1]
+  return _lookup_grad(grad, flat, num_rows, dims, scale, dtype, _grad_workspace(flat, num_rows, dims), device)
 
 
 # -------------------------------------------------------------------------------------------- rows in 4 bits
@@ -207,18 +229,15 @@ class PackedRows:
     if bias is not None:
       _tensor(bias, "bias", 1, (torch.float32,))
       _check(bias.shape[0] == self.num_rows and bias.is_contiguous(), "bias is contiguous, one value a row")
-    _same_device(self.codes, queries, bias)
+    device = _same_device(self.codes, queries, bias)
     q = queries if queries.dim() == 2 else queries[None]
-    stride = _rows(q, "queries")
-    nq, device = q.shape[0], q.device
-    out = torch.empty(nq, self.num_rows, dtype=dtype, device=device)
-    with _on(device):
-      kind = _TYPES[q.dtype]
-      size = _native.packed_scores_workspace(self.num_rows, self.num_dims, self.group, kind, nq)
-      work = _workspace(size, device)
-      _native.packed_scores(self.codes.data_ptr(), self.scales.data_ptr(), _address(self.offsets), _SCALES[self.scales.dtype], self.num_rows,
-                            self.num_dims, self.group, q.data_ptr(), kind, stride, nq, alpha, _address(bias), out.data_ptr(),
-                            _TYPES[dtype], self.num_rows, _address(work), size, _stream(device))
+    nq, kind = q.shape[0], _TYPES[q.dtype]
+    out = q.new_empty((nq, self.num_rows), dtype=dtype)
+    size = _native.packed_scores_workspace(self.num_rows, self.num_dims, self.group, kind, nq)
+    work = _workspace(size, q)
+    _native.packed_scores(self.codes.data_ptr(), self.scales.data_ptr(), _address(self.offsets), _SCALES[self.scales.dtype], self.num_rows,
+                          self.num_dims, self.group, q.data_ptr(), kind, _rows(q, "queries"), nq, alpha, _address(bias), out.data_ptr(),
+                          _TYPES[dtype], self.num_rows, _address(work), size, device, _raw_stream(device))
     return out if queries.dim() == 2 else out[0]
 
   def unpack(self):
@@ -283,12 +302,11 @@ def pack(vectors, group=32, offsets=False, scale_dtype=torch.float16, labels=Non
   stride = _rows(vectors, "vectors")
   _check(group in _GROUPS, "the group is 32, 64 or 128 elements")
   _check(scale_dtype in _SCALES, "scales are float16 or bfloat16")
-  _same_device(vectors)
+  device = _same_device(vectors)
   n, d = vectors.shape
   codes, scales, lows = _empty_packed(n, d, group, offsets, scale_dtype, vectors.device)
-  with _on(vectors.device):
-    _native.pack_rows(vectors.data_ptr(), _TYPES[vectors.dtype], stride, n, d, group, codes.data_ptr(), scales.data_ptr(), _address(lows),
-                      _SCALES[scale_dtype], _stream(vectors.device))
+  _native.pack_rows(vectors.data_ptr(), _TYPES[vectors.dtype], stride, n, d, group, codes.data_ptr(), scales.data_ptr(), _address(lows),
+                    _SCALES[scale_dtype], device, _raw_stream(device))
   return PackedRows(codes, scales, lows, num_dims=d, group=group, labels=labels)
 
 
@@ -303,7 +321,7 @@ def pack_index(index, group=32, offsets=False, scale_dtype=torch.float16):
   device = torch.device("cuda", torch.cuda.current_device())
   n, d = obj.num_data(), obj.num_dims()
   codes, scales, lows = _empty_packed(n, d, group, offsets, scale_dtype, device)
-  obj.pack_items(group, codes.data_ptr(), scales.data_ptr(), _address(lows), _SCALES[scale_dtype], _stream(device))
+  obj.pack_items(group, codes.data_ptr(), scales.data_ptr(), _address(lows), _SCALES[scale_dtype], _raw_stream(device.index))
   labels = obj.get_labels()
   plain = np.array_equal(labels, np.arange(n))
   return PackedRows(codes, scales, lows, num_dims=d, group=group, labels=None if plain else torch.from_numpy(labels).to(device))
@@ -334,19 +352,18 @@ def select_beams(scores, beams, num, normalise=True, finished=None, end=None):
     _check(tuple(finished.shape) == (b, k), "finished has the shape (%d, %d)", b, k)
     _check(beams is not None, "finished beams need what they gathered (beams)")
     _check(isinstance(end, int) and 0 <= end < v, "finished beams need the token that ends a sequence (end)")
-  _same_device(scores, beams, finished)
-  device = scores.device
+  device = _same_device(scores, beams, finished)
   beams = None if beams is None else beams.contiguous()
   finished = None if finished is None else finished.contiguous()
-  totals = torch.empty(b, num, dtype=torch.float32, device=device)
-  parents = torch.empty(b, num, dtype=torch.int32, device=device)
-  tokens = torch.empty(b, num, dtype=torch.int32, device=device)
-  with _on(device):
-    size = _native.select_beams_workspace(_TYPES[scores.dtype], b, k, v, num)
-    work = _workspace(size, device)
-    _native.select_beams(scores.data_ptr(), _TYPES[scores.dtype], scores.stride(0), scores.stride(1), b, k, v, _address(beams),
-                         _address(finished), 0 if end is None else end, int(bool(normalise)), num, totals.data_ptr(), parents.data_ptr(),
-                         tokens.data_ptr(), _address(work), size, _stream(device))
+  totals = scores.new_empty((b, num), dtype=torch.float32)
+  parents = scores.new_empty((b, num), dtype=torch.int32)
+  tokens = scores.new_empty((b, num), dtype=torch.int32)
+  kind = _TYPES[scores.dtype]
+  size = _native.select_beams_workspace(kind, b, k, v, num)
+  work = _workspace(size, scores)
+  _native.select_beams(scores.data_ptr(), kind, scores.stride(0), scores.stride(1), b, k, v, _address(beams), _address(finished),
+                       0 if end is None else end, int(bool(normalise)), num, totals.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                       _address(work), size, device, _raw_stream(device))
   return totals, parents, tokens
 
 
@@ -362,24 +379,24 @@ def reorder_states(states, parents):
   if not states:
     return []
   b, picked = parents.shape
-  first = states[0]
-  outs, sizes = [], []
+  k = states[0].shape[1] if isinstance(states[0], torch.Tensor) and states[0].dim() >= 2 else 0
+  outs, sizes, strides_b, strides_k = [], [], [], []
   for x in states:
     if not isinstance(x, torch.Tensor):
       raise TypeError("states is a list of tensors")
-    _check(x.dim() >= 2 and x.shape[0] == b and x.shape[1] == first.shape[1] and x.shape[1] > 0,
-           "states have the shape [batch, beams, ...]: %s with %d batch entries", tuple(x.shape), b)
+    shape, stride, size = x.shape, x.stride(), x.element_size()
+    _check(len(shape) >= 2 and shape[0] == b and shape[1] == k and k > 0, "states have the shape [batch, beams, ...]: %s with %d batch entries",
+           tuple(shape), b)
     expected = 1
-    for size, stride in zip(reversed(x.shape[2:]), reversed(x.stride()[2:])):
-      _check(size == 1 or stride == expected, "one beam's state has to be contiguous")
-      expected *= size
-    sizes.append(expected * x.element_size())
+    for i in range(len(shape) - 1, 1, -1):
+      _check(shape[i] == 1 or stride[i] == expected, "one beam's state has to be contiguous")
+      expected *= shape[i]
+    sizes.append(expected * size)
+    strides_b.append(stride[0] * size)
+    strides_k.append(stride[1] * size)
   _check(b * picked <= 65535, "at most 65535 states in all")
-  _same_device(parents, *states)
-  for x in states:
-    outs.append(torch.empty(b, picked, *x.shape[2:], dtype=x.dtype, device=x.device))
-  with _on(parents.device):
-    _native.reorder_states([x.data_ptr() for x in states], [x.data_ptr() for x in outs], [x.stride(0) * x.element_size() for x in states],
-                           [x.stride(1) * x.element_size() for x in states], sizes, parents.data_ptr(), parents.stride(0), parents.stride(1),
-                           b, first.shape[1], picked, _stream(parents.device))
+  device = _same_device(parents, *states)
+  outs = [x.new_empty((b, picked, *x.shape[2:])) for x in states]
+  _native.reorder_states([x.data_ptr() for x in states], [x.data_ptr() for x in outs], strides_b, strides_k, sizes, parents.data_ptr(),
+                         parents.stride(0), parents.stride(1), b, k, picked, device, _raw_stream(device))
   return outs

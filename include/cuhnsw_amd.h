@@ -297,7 +297,9 @@ int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, vo
  *   ids: int32, or int64 with ids_64; out: dense [num_ids, num_dims], of the table's type or float32.
  * cuhnsw_lookup_rows_grad: out[v] = scale * sum of grad[t] over the t with ids[t] = v.  In which order the sum is formed
  *   depends on the sizes and the ids alone: the same call gives the same bits.  All of out is written: dense [num_rows, num_dims], of the gradient's type, or
- *   of any where that is float32.  num_ids <= 2^30, num_rows < 2^31 - 1. */
+ *   of any where that is float32.  num_ids <= 2^30, num_rows < 2^31 - 1.
+ * cuhnsw_use_device: makes `device` the thread's current HIP device; *before: the one that was. */
+int cuhnsw_use_device(int device, int* before);
 int cuhnsw_lookup_rows(const void* table, int table_type, long long num_rows, long long row_stride, int num_dims, const void* ids,
                        int ids_64, long long num_ids, float scale, void* out, int out_type, void* stream);
 long long cuhnsw_lookup_grad_workspace(long long num_ids, long long num_rows, int num_dims);

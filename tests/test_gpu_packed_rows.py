@@ -112,7 +112,7 @@ def test_scores_are_written_where_they_belong_and_nowhere_else():
   size = cuhnsw_bind.packed_scores_workspace(n, d, 32, 0, nq)
   work = torch.empty(size + 1, dtype=torch.uint8, device="cuda")
   cuhnsw_bind.packed_scores(packed.codes.data_ptr(), packed.scales.data_ptr(), 0, 1, n, d, 32, q.data_ptr(), 0, d, nq, 1.0, 0,
-                            out[1].data_ptr(), 0, 100, work.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+                            out[1].data_ptr(), 0, 100, work.data_ptr(), size, 0, torch.cuda.current_stream().cuda_stream)
   assert torch.equal(out[1:-1, :n], want)
   assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[1:-1, n:] == 7).all()
 
