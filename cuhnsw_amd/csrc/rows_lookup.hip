@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortInput in, 
     before[j] = 0;
     if (j >= per_thread || d >= digits) continue;
     int all = 0;
-#pragma unroll 8
+#pragma unroll 32
     for (int b = 0; b < (int)gridDim.x; ++b) {
       const int n = counts[b * digits + d];
       before[j] += b < (int)blockIdx.x ? n : 0;
@@ -220,51 +220,49 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortInput in, 
 // than that.  Which sum is formed in which order depends on sizes and ids alone.
 constexpr int kLong = 64, kFew = 2048, kMostRows = 128;
 
-// sum of the vector at d over the items [from, to), in order
-template <int VE, typename F>
-__device__ inline void sum_items(int from, int to, F&& item, float (&sum)[VE]) {
+// sum of the vectors of the items [from, to), in order, up to eight of them in flight; where(i): item i's address
+template <typename T, int VE, int N, typename F>
+__device__ inline void add_items(int from, int count, F&& where, float (&sum)[VE]) {
+  LoosePack<T, VE> x[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < count) x[j] = *where(from + j);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < count)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) sum[e] += widen(x[j].at[e]);
+}
+template <typename T, int VE, typename F>
+__device__ inline void sum_items(int from, int to, F&& where, float (&sum)[VE]) {
 #pragma unroll
   for (int e = 0; e < VE; ++e) sum[e] = 0.f;
   int i = from;
-  for (; i + 4 <= to; i += 4) {
-    float x[4][VE];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) item(i + j, x[j]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) sum[e] += x[j][e];
+  for (; i + 8 <= to; i += 8) add_items<T, VE, 8>(i, 8, where, sum);
+  if (i + 4 <= to) {
+    add_items<T, VE, 4>(i, 4, where, sum);
+    i += 4;
   }
-  for (; i < to; ++i) {
-    float x[VE];
-    item(i, x);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) sum[e] += x[e];
-  }
+  if (i < to) add_items<T, VE, 3>(i, to - i, where, sum);
 }
 
-// The same by the whole workgroup, a contiguous part of the items for every group of lanes; the first group has the sum.
-// parts: 256 x VE places in LDS.
-template <int VE, typename F>
-__device__ inline void sum_items_together(int items, int lanes, F&& item, float (&sum)[VE], float* parts) {
+// The same by the whole workgroup, a contiguous part of the items for every group of lanes; the first group adds the parts to
+// what it has.  parts: 256 x VE places in LDS.
+template <typename T, int VE, typename F>
+__device__ inline void sum_items_together(int items, int lanes, F&& where, float (&sum)[VE], float* parts) {
   const int groups = 256 / lanes, group = threadIdx.x / lanes, share = (items + groups - 1) / groups;
-  sum_items<VE>(min(items, group * share), min(items, (group + 1) * share), item, sum);
+  float mine[VE];
+  sum_items<T, VE>(min(items, group * share), min(items, (group + 1) * share), where, mine);
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < VE; ++e) parts[threadIdx.x * VE + e] = sum[e];
+  for (int e = 0; e < VE; ++e) parts[threadIdx.x * VE + e] = mine[e];
   __syncthreads();
   if (group == 0)
-    for (int g = 1; g < groups; ++g)
+    for (int g = 0; g < min(groups, items); ++g)
 #pragma unroll
       for (int e = 0; e < VE; ++e) sum[e] += parts[(g * lanes + threadIdx.x) * VE + e];
 }
 
-template <typename T, int VE>
-__device__ inline void fetch(const T* from, float (&x)[VE]) {
-  const LoosePack<T, VE> p = *reinterpret_cast<const LoosePack<T, VE>*>(from);
-#pragma unroll
-  for (int e = 0; e < VE; ++e) x[e] = widen(p.at[e]);
-}
 template <typename U, int VE>
 __device__ inline void store(U* to, const float (&x)[VE], float scale) {
   LoosePack<U, VE> p;
@@ -280,59 +278,64 @@ struct GradArgs {
   int ids_64;
   const int *keys, *places;  // many: in order
   float* long_sums;          // [num_ids / kLong, num_dims]: sums of the stretches that are one id's alone
+  int* bounds;               // where every workgroup's rows begin in the sorted list, and the end of the last one's
+  int num_stretches, num_blocks;
   int num_ids, num_rows, num_dims;
   float scale;
   void* out;
   int lanes, rows;  // lanes that share a row, rows of a workgroup
 };
 
+// Stretches of the sorted list that are one id's alone; and, by the workgroups behind those, where the rows of grad_kernel's
+// workgroups begin: a search for each thread, which would be every one's first wait there.
 template <typename T, int VE>
 __global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
   __shared__ float parts[256 * VE];
+  if ((int)blockIdx.x >= a.num_stretches) {
+    const int i = (blockIdx.x - a.num_stretches) * 256 + threadIdx.x;
+    if (i > a.num_blocks) return;
+    const int row = (int)min((long long)i * a.rows, (long long)a.num_rows);
+    int low = 0, high = a.num_ids;
+    while (low < high) {
+      const int mid = (low + high) >> 1;
+      if (a.keys[mid] < row) low = mid + 1;
+      else high = mid;
+    }
+    a.bounds[i] = low;
+    return;
+  }
   const int first = blockIdx.x * kLong, key = a.keys[first];
   if (key >= a.num_rows || a.keys[first + kLong - 1] != key) return;
   const int lane = threadIdx.x & (a.lanes - 1), vectors = vectors_of<VE>(a.num_dims);
   const T* grad = static_cast<const T*>(a.grad);
   for (int v0 = 0; v0 < vectors; v0 += a.lanes) {
     const int d = vector_at<VE>(min(v0 + lane, vectors - 1), a.num_dims);
-    float sum[VE];
-    sum_items_together<VE>(kLong, a.lanes, [&](int i, float (&x)[VE]) { fetch<T, VE>(grad + (long long)a.places[first + i] * a.grad_stride + d, x); },
-                           sum, parts);
+    float sum[VE] = {};
+    sum_items_together<T, VE>(kLong, a.lanes, [&](int i) {
+      return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)a.places[first + i] * a.grad_stride + d);
+    }, sum, parts);
     if (threadIdx.x < a.lanes) store<float, VE>(a.long_sums + (long long)blockIdx.x * a.num_dims + d, sum, 1.f);
   }
-}
-
-// by a wavefront: the first place in [0, n) whose key is at least `key`
-__device__ inline int lower_bound(const int* keys, int n, int key) {
-  const int lane = threadIdx.x & 63;
-  int low = 0, size = n;
-  while (size > 0) {
-    const int step = (size + 63) / 64, at = low + (lane + 1) * step - 1;
-    const int less = __popcll(__ballot((lane + 1) * (long long)step <= size && keys[at] < key));
-    low += less * step;
-    size = min(step - 1, size - less * step);
-  }
-  return low;
 }
 
 template <typename T, typename U, int VE, bool FEW>
 __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
   __shared__ int first[kMostRows], last[kMostRows];
-  __shared__ int bounds[2];
+  __shared__ int picked_count;
   __shared__ float parts[256 * VE];
-  __shared__ uint64_t picked[FEW ? kFew : 1];
-  __shared__ int in_order[FEW ? kFew : 1];
+  extern __shared__ uint64_t picked[];  // few ids: [num_ids], and their places in order behind them
+  int* in_order = reinterpret_cast<int*>(picked + (FEW ? a.num_ids : 0));
   const int tid = threadIdx.x, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.num_rows - row0);
   for (int r = tid; r < rows; r += 256) first[r] = last[r] = 0;
   if (FEW) {
-    if (tid == 0) bounds[0] = 0;
+    if (tid == 0) picked_count = 0;
     __syncthreads();
     for (int i = tid; i < a.num_ids; i += 256) {
       const long long r = id_at(a.ids, a.ids_64, i) - row0;
-      if (r >= 0 && r < rows) picked[atomicAdd(&bounds[0], 1)] = (uint64_t)r << 32 | (uint32_t)i;
+      if (r >= 0 && r < rows) picked[atomicAdd(&picked_count, 1)] = (uint64_t)r << 32 | (uint32_t)i;
     }
     __syncthreads();
-    const int count = bounds[0];
+    const int count = picked_count;
     for (int i = tid; i < count; i += 256) {
       const uint64_t mine = picked[i];
       int rank = 0, same = 0, under = 0;
@@ -349,15 +352,12 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
       }
     }
   } else {
-    if (tid < 128) {
-      const int at = lower_bound(a.keys, a.num_ids, tid < 64 ? row0 : row0 + rows);
-      if ((tid & 63) == 0) bounds[tid >> 6] = at;
-    }
+    const int begin = a.bounds[blockIdx.x], end = a.bounds[blockIdx.x + 1];
     __syncthreads();
-    for (int i = bounds[0] + tid; i < bounds[1]; i += 256) {
+    for (int i = begin + tid; i < end; i += 256) {
       const int key = a.keys[i];
-      if (i == bounds[0] || a.keys[i - 1] != key) first[key - row0] = i;
-      if (i + 1 == bounds[1] || a.keys[i + 1] != key) last[key - row0] = i + 1;
+      if (i == begin || a.keys[i - 1] != key) first[key - row0] = i;
+      if (i + 1 == end || a.keys[i + 1] != key) last[key - row0] = i + 1;
     }
   }
   __syncthreads();
@@ -374,8 +374,8 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
     for (int v = lane; v < vectors; v += a.lanes) {
       const int d = vector_at<VE>(v, a.num_dims);
       float sum[VE];
-      sum_items<VE>(from, to, [&](int i, float (&x)[VE]) {
-        fetch<T, VE>(grad + (long long)(FEW ? in_order[i] : a.places[i]) * a.grad_stride + d, x);
+      sum_items<T, VE>(from, to, [&](int i) {
+        return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)(FEW ? in_order[i] : a.places[i]) * a.grad_stride + d);
       }, sum);
       store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
     }
@@ -389,14 +389,14 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
     const int head = FEW ? to - from : whole * kLong - from, stretches = FEW ? 0 : ends - whole, tail = FEW ? 0 : to - ends * kLong;
     for (int v0 = 0; v0 < vectors; v0 += a.lanes) {
       const int d = vector_at<VE>(min(v0 + lane, vectors - 1), a.num_dims);
-      float sum[VE];
-      sum_items_together<VE>(head + stretches + tail, a.lanes, [&](int i, float (&x)[VE]) {
-        if (!FEW && i >= head && i < head + stretches) {
-          fetch<float, VE>(a.long_sums + (long long)(whole + i - head) * a.num_dims + d, x);
-        } else {
-          const int at = i < head ? from + i : ends * kLong + i - head - stretches;
-          fetch<T, VE>(grad + (long long)(FEW ? in_order[at] : a.places[at]) * a.grad_stride + d, x);
-        }
+      float sum[VE] = {};
+      if (stretches > 0)
+        sum_items_together<float, VE>(stretches, a.lanes, [&](int i) {
+          return reinterpret_cast<const LoosePack<float, VE>*>(a.long_sums + (long long)(whole + i) * a.num_dims + d);
+        }, sum, parts);
+      sum_items_together<T, VE>(head + tail, a.lanes, [&](int i) {
+        const int at = i < head ? from + i : ends * kLong + i - head;
+        return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)(FEW ? in_order[at] : a.places[at]) * a.grad_stride + d);
       }, sum, parts);
       if (tid < a.lanes) store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
     }
@@ -406,8 +406,9 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
 struct GradScratch {
   int *keys[2], *places[2], *counts;
   float* long_sums;
+  int* bounds;
   size_t bytes;
-  GradScratch(void* memory, long long num_ids, int num_dims, const SortPlan& p) {
+  GradScratch(void* memory, long long num_ids, long long num_rows, int num_dims, const SortPlan& p) {
     WorkspaceParts s(memory);
     for (int i = 0; i < 2; ++i) {
       keys[i] = s.part<int>((size_t)num_ids);
@@ -415,6 +416,7 @@ struct GradScratch {
     }
     counts = s.part<int>((size_t)p.blocks << p.bits);
     long_sums = s.part<float>((size_t)(num_ids / kLong) * num_dims);
+    bounds = s.part<int>((size_t)num_rows + 2);  // (at least a row for every workgroup)
     bytes = s.used();
   }
 };
@@ -449,7 +451,7 @@ int cuhnsw_lookup_rows(const void* table, int table_type, long long num_rows, lo
 
 long long cuhnsw_lookup_grad_workspace(long long num_ids, long long num_rows, int num_dims) {
   if (num_ids <= kFew || num_ids > 1 << 30 || num_rows <= 0 || num_rows >= 0x7fffffff || num_dims <= 0) return 0;
-  return (long long)GradScratch(nullptr, num_ids, num_dims, sort_plan(num_ids, num_rows)).bytes;
+  return (long long)GradScratch(nullptr, num_ids, num_rows, num_dims, sort_plan(num_ids, num_rows)).bytes;
 }
 
 int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stride, const void* ids, int ids_64, long long num_ids,
@@ -476,7 +478,7 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
     const bool few = num_ids <= kFew;
     if (!few) {
       const SortPlan p = sort_plan(num_ids, num_rows);
-      const GradScratch w(workspace, num_ids, num_dims, p);
+      const GradScratch w(workspace, num_ids, num_rows, num_dims, p);
       want(workspace && workspace_bytes >= (long long)w.bytes, "lookup gradient: the workspace is too small");
       for (int pass = 0; pass < p.passes; ++pass) {
         const SortInput in{ids, ids_64, (int)num_rows, pass ? w.keys[(pass - 1) & 1] : nullptr, pass ? w.places[(pass - 1) & 1] : nullptr};
@@ -488,6 +490,8 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
       g.keys = w.keys[(p.passes - 1) & 1];
       g.places = w.places[(p.passes - 1) & 1];
       g.long_sums = w.long_sums;
+      g.bounds = w.bounds;
+      g.num_stretches = (int)(num_ids / kLong);
     }
     with_type(grad_type, [&](auto* t) {
       with_type(out_type, [&](auto* u) {
@@ -501,11 +505,12 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
             const int groups = 256 / g.lanes;
             const long long bytes = (long long)num_dims * (sizeof(U) + sizeof(T) * (num_ids / num_rows));
             g.rows = (int)std::min<long long>(kMostRows, std::max<long long>(groups, 32768 / bytes / groups * groups));
-            const dim3 grid((unsigned)((num_rows + g.rows - 1) / g.rows));
+            g.num_blocks = (int)((num_rows + g.rows - 1) / g.rows);
+            const dim3 grid((unsigned)g.num_blocks);
             if (few) {
-              hipLaunchKernelGGL((grad_kernel<T, U, VE, true>), grid, dim3(256), 0, s, g);
+              hipLaunchKernelGGL((grad_kernel<T, U, VE, true>), grid, dim3(256), (size_t)num_ids * 12, s, g);
             } else {
-              hipLaunchKernelGGL((grad_long_kernel<T, VE>), dim3((unsigned)(num_ids / kLong)), dim3(256), 0, s, g);
+              hipLaunchKernelGGL((grad_long_kernel<T, VE>), dim3((unsigned)(g.num_stretches + g.num_blocks / 256 + 1)), dim3(256), 0, s, g);
               hipLaunchKernelGGL((grad_kernel<T, U, VE, false>), grid, dim3(256), 0, s, g);
             }
           });
