@@ -214,11 +214,11 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortInput in, 
 
 // ------------------------------------------------------------------------------------------- gradient
 // A workgroup has a stretch of rows and the (key, place) pairs of theirs, in order: out of the sorted list, or, where there
-// are few ids, picked out of all of them and ranked in LDS (one launch, and nothing is sorted).  A row of up to kLong places is a
-// group of lanes' own; the places of a longer one are divided among all groups of the workgroup.  In the sorted list
+// are few ids, picked out of all of them and ranked in LDS (one launch, and nothing is sorted).  A row of up to kTogether places
+// is a group of lanes' own; the places of a longer one are divided among all groups of the workgroup.  In the sorted list
 // stretches of kLong places of one id have been summed before (grad_long_kernel), so that no row is much longer
 // than that.  Which sum is formed in which order depends on sizes and ids alone.
-constexpr int kLong = 64, kFew = 2048, kMostRows = 128;
+constexpr int kLong = 64, kTogether = 16, kFew = 2048, kMostRows = 128;
 
 // sum of the vectors of the items [from, to), in order, up to eight of them in flight; where(i): item i's address
 template <typename T, int VE, int N, typename F>
@@ -321,12 +321,14 @@ __global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
 template <typename T, typename U, int VE, bool FEW>
 __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
   __shared__ int first[kMostRows], last[kMostRows];
+  __shared__ int long_rows[kMostRows], long_count;
   __shared__ int picked_count;
   __shared__ float parts[256 * VE];
   extern __shared__ uint64_t picked[];  // few ids: [num_ids], and their places in order behind them
   int* in_order = reinterpret_cast<int*>(picked + (FEW ? a.num_ids : 0));
   const int tid = threadIdx.x, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.num_rows - row0);
   for (int r = tid; r < rows; r += 256) first[r] = last[r] = 0;
+  if (tid == 0) long_count = 0;
   if (FEW) {
     if (tid == 0) picked_count = 0;
     __syncthreads();
@@ -364,11 +366,10 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
   const T* grad = static_cast<const T*>(a.grad);
   U* out = static_cast<U*>(a.out) + (long long)row0 * a.num_dims;
   const int lane = tid & (a.lanes - 1), groups = 256 / a.lanes, vectors = vectors_of<VE>(a.num_dims);
-  bool any_long = false;
   for (int r = tid / a.lanes; r < rows; r += groups) {
     const int from = first[r], to = last[r];
-    if (to - from > kLong) {
-      any_long = true;
+    if (to - from > kTogether) {
+      if (lane == 0) long_rows[atomicAdd(&long_count, 1)] = r;
       continue;
     }
     for (int v = lane; v < vectors; v += a.lanes) {
@@ -380,13 +381,13 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
       store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
     }
   }
-  if (!__syncthreads_or(any_long)) return;
-  for (int r = 0; r < rows; ++r) {
-    const int from = first[r], to = last[r];
-    if (to - from <= kLong) continue;
+  __syncthreads();
+  for (int l = 0; l < long_count; ++l) {
+    const int r = long_rows[l], from = first[r], to = last[r];
     // its places up to the first whole stretch, the whole stretches, the places behind them
-    const int whole = FEW ? to : (from + kLong - 1) / kLong, ends = FEW ? to : to / kLong;
-    const int head = FEW ? to - from : whole * kLong - from, stretches = FEW ? 0 : ends - whole, tail = FEW ? 0 : to - ends * kLong;
+    const int whole = (from + kLong - 1) / kLong, ends = to / kLong;
+    const bool any_whole = !FEW && whole < ends;
+    const int head = any_whole ? whole * kLong - from : to - from, stretches = any_whole ? ends - whole : 0, tail = any_whole ? to - ends * kLong : 0;
     for (int v0 = 0; v0 < vectors; v0 += a.lanes) {
       const int d = vector_at<VE>(min(v0 + lane, vectors - 1), a.num_dims);
       float sum[VE] = {};
