@@ -26,6 +26,23 @@ template <int VE>
 __device__ inline int vector_at(int v, int num_dims) {
   return min(v * VE, num_dims - VE);
 }
+// A large result goes past the caches, whose lines would otherwise all be written back when the kernel ends.
+constexpr long long kStreamedFrom = 64ll << 20;
+template <bool STREAMED, typename U, int VE>
+__device__ inline void store_result(U* to, const LoosePack<U, VE>& p) {
+  if constexpr (STREAMED && sizeof(p) == 16) {
+    typedef uint32_t vector_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t loose_t __attribute__((ext_vector_type(4), aligned(2)));
+    __builtin_nontemporal_store(__builtin_bit_cast(vector_t, p), reinterpret_cast<loose_t*>(to));
+  } else {
+    *reinterpret_cast<LoosePack<U, VE>*>(to) = p;
+  }
+}
+template <typename F>
+void with_flag(bool flag, F&& f) {
+  if (flag) f(std::true_type());
+  else f(std::false_type());
+}
 // lanes that share a row: the power of two that its vectors fill at least half of, a wavefront at most
 inline int lanes_of(int vectors) {
   int lanes = 1;
@@ -42,7 +59,7 @@ void with_vector(int num_dims, F&& f) {
 
 // ---------------------------------------------------------------------------------------------- lookup
 // Bound by memory: each row is fetched once and written once, four rows of a lane's in flight.
-template <typename T, typename U, int VE>
+template <typename T, typename U, int VE, bool STREAMED>
 __global__ void __launch_bounds__(256) lookup_kernel(const T* table, long long num_rows, long long row_stride, int num_dims,
                                                      const void* ids, int ids_64, long long num_ids, float scale, U* out, int lanes) {
   constexpr int kAtOnce = 4;
@@ -68,7 +85,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T* table, long long n
         LoosePack<U, VE> y;
 #pragma unroll
         for (int e = 0; e < VE; ++e) y.at[e] = narrow<U>(from[j] ? scale * widen(x[j].at[e]) : 0.f);
-        *reinterpret_cast<LoosePack<U, VE>*>(out + t * num_dims + d) = y;
+        store_result<STREAMED>(out + t * num_dims + d, y);
       }
     }
   }
@@ -85,9 +102,11 @@ void launch_lookup(const LookupArgs& a, hipStream_t stream) {
           constexpr int VE = decltype(ve)::value;
           const int lanes = lanes_of(vectors_of<VE>(a.num_dims)), groups = 256 / lanes;
           const long long blocks = std::min<long long>((a.num_ids + groups - 1) / groups, 1 << 20);
-          hipLaunchKernelGGL((lookup_kernel<T, U, VE>), dim3((unsigned)(blocks <= 2048 ? blocks : (blocks + 3) / 4)), dim3(256), 0, stream,
-                             static_cast<const T*>(a.table), a.num_rows, a.row_stride, a.num_dims, a.ids, a.ids_64, a.num_ids, a.scale,
-                             static_cast<U*>(a.out), lanes);
+          with_flag(a.num_ids * a.num_dims * (long long)sizeof(U) >= kStreamedFrom, [&](auto streamed) {
+            hipLaunchKernelGGL((lookup_kernel<T, U, VE, decltype(streamed)::value>), dim3((unsigned)(blocks <= 2048 ? blocks : (blocks + 3) / 4)),
+                               dim3(256), 0, stream, static_cast<const T*>(a.table), a.num_rows, a.row_stride, a.num_dims, a.ids, a.ids_64,
+                               a.num_ids, a.scale, static_cast<U*>(a.out), lanes);
+          });
         });
       } else {
         throw std::runtime_error("lookup: the result has the table's type or is float32");
@@ -263,12 +282,12 @@ __device__ inline void sum_items_together(int items, int lanes, F&& where, float
       for (int e = 0; e < VE; ++e) sum[e] += parts[(g * lanes + threadIdx.x) * VE + e];
 }
 
-template <typename U, int VE>
+template <bool STREAMED, typename U, int VE>
 __device__ inline void store(U* to, const float (&x)[VE], float scale) {
   LoosePack<U, VE> p;
 #pragma unroll
   for (int e = 0; e < VE; ++e) p.at[e] = narrow<U>(scale * x[e]);
-  *reinterpret_cast<LoosePack<U, VE>*>(to) = p;
+  store_result<STREAMED>(to, p);
 }
 
 struct GradArgs {
@@ -314,11 +333,11 @@ __global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
     sum_items_together<T, VE>(kLong, a.lanes, [&](int i) {
       return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)a.places[first + i] * a.grad_stride + d);
     }, sum, parts);
-    if (threadIdx.x < a.lanes) store<float, VE>(a.long_sums + (long long)blockIdx.x * a.num_dims + d, sum, 1.f);
+    if (threadIdx.x < a.lanes) store<false>(a.long_sums + (long long)blockIdx.x * a.num_dims + d, sum, 1.f);
   }
 }
 
-template <typename T, typename U, int VE, bool FEW>
+template <typename T, typename U, int VE, bool FEW, bool STREAMED>
 __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
   __shared__ int first[kMostRows], last[kMostRows];
   __shared__ int long_rows[kMostRows], long_count;
@@ -378,7 +397,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
       sum_items<T, VE>(from, to, [&](int i) {
         return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)(FEW ? in_order[i] : a.places[i]) * a.grad_stride + d);
       }, sum);
-      store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
+      store<STREAMED>(out + (long long)r * a.num_dims + d, sum, a.scale);
     }
   }
   __syncthreads();
@@ -399,7 +418,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
         const int at = i < head ? from + i : ends * kLong + i - head;
         return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)(FEW ? in_order[at] : a.places[at]) * a.grad_stride + d);
       }, sum, parts);
-      if (tid < a.lanes) store<U, VE>(out + (long long)r * a.num_dims + d, sum, a.scale);
+      if (tid < a.lanes) store<STREAMED>(out + (long long)r * a.num_dims + d, sum, a.scale);
     }
   }
 }
@@ -508,12 +527,13 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
             g.rows = (int)std::min<long long>(kMostRows, std::max<long long>(groups, 32768 / bytes / groups * groups));
             g.num_blocks = (int)((num_rows + g.rows - 1) / g.rows);
             const dim3 grid((unsigned)g.num_blocks);
-            if (few) {
-              hipLaunchKernelGGL((grad_kernel<T, U, VE, true>), grid, dim3(256), (size_t)num_ids * 12, s, g);
-            } else {
+            if (!few)
               hipLaunchKernelGGL((grad_long_kernel<T, VE>), dim3((unsigned)(g.num_stretches + g.num_blocks / 256 + 1)), dim3(256), 0, s, g);
-              hipLaunchKernelGGL((grad_kernel<T, U, VE, false>), grid, dim3(256), 0, s, g);
-            }
+            with_flag(num_rows * num_dims * (long long)sizeof(U) >= kStreamedFrom, [&](auto streamed) {
+              constexpr bool kStreamed = decltype(streamed)::value;
+              if (few) hipLaunchKernelGGL((grad_kernel<T, U, VE, true, kStreamed>), grid, dim3(256), (size_t)num_ids * 12, s, g);
+              else hipLaunchKernelGGL((grad_kernel<T, U, VE, false, kStreamed>), grid, dim3(256), 0, s, g);
+            });
           });
         } else {
           throw std::runtime_error("lookup gradient: the gradient has the table's type or is float32");
