@@ -113,10 +113,14 @@ __device__ inline int keep_best(uint64_t* keys, int count, int most) {
 }
 
 // Pass over a row's scores: NV vectors of 16 bytes for each thread are a tile, and the next tile is asked for before the one
-// at hand is looked at.  The first tile gives a value that `num` of its scores reach; what is not below it goes to a list in LDS,
-// which is cut down to its best after that tile and whenever it has grown long: what comes later has to reach the worst of
-// them.  Where a tile would overflow the list (scores in an order that is hard) it enters a score of each thread at a time.
-template <typename T, int NV>
+// at hand is looked at.  The first tile gives a value that `num` of its scores reach; a score that is not below it goes to a list in
+// LDS.  After 1, 2, 4, 8... tiles the list is cut down to its best, and what comes later has to reach the worst of them: a hundred
+// or so enter between two cuts, and between two cuts the wavefronts do not wait for each other.  Where a list would
+// overflow meanwhile (scores in an order that is hard) those tiles are gone over again, a score of each thread at a time.
+//
+// What a score costs: its conversion, a comparison, and normalised the maximum, a subtraction, a product, the exponential (of four
+// times the cost) and an addition.
+template <typename T, int NV, bool NORMALISE>
 __global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) {
   constexpr int VE = 16 / sizeof(T), EACH = NV * VE;
   typedef LoosePack<T, VE> Vector;
@@ -150,97 +154,92 @@ __global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) 
     }
   };
   int have = 0;
-  uint64_t bar_key = 0;   // what a key has to be above, once the list was cut
-  float bar = -INFINITY;  // what a score has to reach
-  float top = -INFINITY, sum = 0.f;
-  int first = part * a.each * kTile;
-  const int tiles = max(part == 0 ? 1 : 0, first < vectors ? min(a.each, (vectors - first + kTile - 1) / kTile) : 0);
-  const int extra_place = vectors * VE + tid;
-  float extra = part == 0 && tid < tail ? score_at(widen(x[extra_place])) : -INFINITY;
-  Vector next[NV];
-  if (tiles > 0) load(first, next);
-  for (int t = 0; t < tiles; ++t, first += kTile) {
-    float v[EACH];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) v[i] = score_at(widen(next[i / VE].at[i % VE]));
-    if (t + 1 < tiles) load(first + kTile, next);
-    float largest = extra;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) largest = fmaxf(largest, v[i]);
-    if (a.normalise) {
-      constexpr float kLog2e = 1.44269504f;
-      if (largest > top) {
-        sum *= __builtin_amdgcn_exp2f((top - largest) * kLog2e);
-        top = largest;
-      }
-      const float base = top == -INFINITY ? 0.f : top;
-      const float before = sum;
-      sum += __builtin_amdgcn_exp2f((extra - base) * kLog2e);
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);
-      if (top == INFINITY) {  // (beside an infinite one only the infinite ones count)
-        sum = before + (extra == INFINITY ? 1.f : 0.f);
-        for (int i = 0; i < EACH; ++i) sum += v[i] == INFINITY ? 1.f : 0.f;
-      }
+  uint64_t bar_key = 0;  // what a key has to be above, once the list was cut
+  float bar = 0.f;       // what a score has to reach (always finite: -infinity and NaN never do)
+  constexpr float kLowest = -3.402823466e38f;
+  auto cut = [&] {
+    have = keep_best(kept, have, a.most);
+    if (have == a.most) {
+      bar_key = kept[have - 1];
+      bar = fmaxf(key_value(bar_key), kLowest);
     }
-    if (t == 0) bar = reached_by(largest, a.most, INFINITY, shared);
-    uint32_t in = 0;  // which of the thread's scores go to the list
-    int at = 0;
-    if (largest >= bar && largest > -INFINITY) {
+    if (tid == 0) filled = have;
+    __syncthreads();
+  };
+  float top = -INFINITY, sum = 0.f;
+  const int first_vector = part * a.each * kTile;
+  const int tiles = max(part == 0 ? 1 : 0, first_vector < vectors ? min(a.each, (vectors - first_vector + kTile - 1) / kTile) : 0);
+  const int extra_place = vectors * VE + tid;
+  const float extra = part == 0 && tid < tail ? score_at(widen(x[extra_place])) : -INFINITY;
+  auto place = [&](int t, int i) { return (first_vector + t * kTile + i / VE * kThreads + tid) * VE + i % VE; };
+  Vector next[NV];
+  if (tiles > 0) load(first_vector, next);
+  for (int t = 0, segment = 1; t < tiles; segment = t) {
+    const int begin = t, end = min(tiles, t + segment);
+    for (; t < end; ++t) {
+      float v[EACH];
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) in |= v[i] >= bar && v[i] > -INFINITY ? 1u << i : 0u;
-      in |= extra >= bar && extra > -INFINITY ? 1u << EACH : 0u;
-      at = atomicAdd(&filled, __popc(in));
+      for (int i = 0; i < EACH; ++i) v[i] = NORMALISE ? score_at(widen(next[i / VE].at[i % VE])) : widen(next[i / VE].at[i % VE]);
+      if (t + 1 < tiles) load(first_vector + (t + 1) * kTile, next);
+      if (NORMALISE || t == 0) {
+        float largest = t == 0 ? extra : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) largest = fmaxf(largest, v[i]);
+        if (NORMALISE) {
+          constexpr float kLog2e = 1.44269504f;
+          if (largest > top) {
+            sum *= __builtin_amdgcn_exp2f((top - largest) * kLog2e);
+            top = largest;
+          }
+          const float base = top == -INFINITY ? 0.f : top, before = sum;
+          if (t == 0) sum += __builtin_amdgcn_exp2f((extra - base) * kLog2e);
+#pragma unroll
+          for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);
+          if (top == INFINITY) {  // (beside an infinite one only the infinite ones count)
+            sum = before + (t == 0 && extra == INFINITY ? 1.f : 0.f);
+            for (int i = 0; i < EACH; ++i) sum += v[i] == INFINITY ? 1.f : 0.f;
+          }
+        }
+        if (t == 0) bar = fmaxf(reached_by(largest, a.most, INFINITY, shared), kLowest);
+      }
+      auto offer = [&](float value, int at_row) {
+        const bool in = value >= bar;
+        const unsigned long long with = __ballot(in);
+        if (with) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&filled, __popcll(with));
+          at = __shfl(at, 0) + __popcll(with & ((1ull << lane) - 1));
+          if (in && at < kKept) kept[at] = order_key(value, (uint32_t)at_row);
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) offer(v[i], place(t, i));
+      if (t == 0) offer(extra, extra_place);
     }
     __syncthreads();
-    const int now = filled;
-    auto place = [&](int i) { return (first + i / VE * kThreads + tid) * VE + i % VE; };
-    if (now <= kKept) {
-      if (in) {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i)
-          if (in >> i & 1) kept[at++] = order_key(v[i], (uint32_t)place(i));
-        if (in >> EACH & 1) kept[at++] = order_key(extra, (uint32_t)extra_place);
-      }
-      have = now;
-      __syncthreads();
-      if (t + 1 < tiles && (t == 0 ? have > a.most : have > 2 * kThreads)) {  // what comes after has to beat the worst of the best so far
-        have = keep_best(kept, have, a.most);
-        if (have == a.most) {
-          bar_key = kept[have - 1];
-          bar = key_value(bar_key);
-        }
-        if (tid == 0) filled = have;
-        __syncthreads();
-      }
+    if (filled <= kKept) {
+      have = filled;
     } else {
-#pragma unroll 1
-      for (int i = 0; i <= EACH; ++i) {
-        if (i == 0 || have + kThreads > kKept) {
-          have = keep_best(kept, have, a.most);
-          if (have == a.most) {
-            bar_key = kept[have - 1];
-            bar = key_value(bar_key);
-          }
-          if (tid == 0) filled = have;
+      for (int again = begin; again < end; ++again)
+        for (int i = 0; i < EACH + (again == 0 ? 1 : 0); ++i) {
+          if ((again == begin && i == 0) || have + kThreads > kKept) cut();
+          const int at_row = i < EACH ? place(again, i) : extra_place;
+          const bool there = i < EACH ? first_vector + again * kTile + i / VE * kThreads + tid < vectors : part == 0 && tid < tail;
+          const float value = there ? score_at(widen(x[at_row])) : -INFINITY;
+          const uint64_t key = order_key(value, (uint32_t)at_row);
+          if (value > -INFINITY && key > bar_key) kept[atomicAdd(&filled, 1)] = key;
+          __syncthreads();
+          have = filled;
           __syncthreads();
         }
-        if (in >> i & 1) {
-          const int at_row = i < EACH ? place(i) : extra_place;
-          const uint64_t key = order_key(score_at(widen(x[at_row])), (uint32_t)at_row);
-          if (key > bar_key) kept[atomicAdd(&filled, 1)] = key;
-        }
-        __syncthreads();
-        have = filled;
-        __syncthreads();
-      }
     }
-    extra = -INFINITY;
+    if (t < tiles && have > a.most) cut();
+    __syncthreads();
   }
   have = keep_best(kept, have, a.most);
   uint64_t* list = a.lists + (long long)blockIdx.x * a.most;
   for (int i = tid; i < a.most; i += kThreads) list[i] = i < have ? kept[i] : 0;
-  if (a.normalise) {
+  if (NORMALISE) {
     float most = top;
     for (int step = 32; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
     if (lane == 0) shared[wave] = most;
@@ -540,8 +539,10 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const dim3 grid((unsigned)(rows * p.parts));
-      if (p.small) hipLaunchKernelGGL((select_part_kernel<T, 1>), grid, dim3(kThreads), 0, s, a);
-      else hipLaunchKernelGGL((select_part_kernel<T, sizeof(T)>), grid, dim3(kThreads), 0, s, a);
+      if (p.small && normalise) hipLaunchKernelGGL((select_part_kernel<T, 1, true>), grid, dim3(kThreads), 0, s, a);
+      else if (p.small) hipLaunchKernelGGL((select_part_kernel<T, 1, false>), grid, dim3(kThreads), 0, s, a);
+      else if (normalise) hipLaunchKernelGGL((select_part_kernel<T, sizeof(T), true>), grid, dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((select_part_kernel<T, sizeof(T), false>), grid, dim3(kThreads), 0, s, a);
     });
     hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)num_batch), dim3(kThreads), (size_t)num_beams * 16, s, a);
     HIP_CHECK(hipGetLastError());
