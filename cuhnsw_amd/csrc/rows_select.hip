@@ -16,6 +16,7 @@
 namespace cuhnsw_amd {
 
 constexpr int kMostNum = 256, kMostBeams = 1024, kMostLists = 4096;
+constexpr int kMostCandidates = 16384;  // in the lists of a batch entry: what one workgroup holds in registers
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kKept = 2048;  // candidates a workgroup holds in LDS
 
@@ -49,22 +50,20 @@ __device__ inline float score_at(float x) { return fmaxf(x, -INFINITY); }  // (o
 
 // The num-th largest of the workgroup's threads' values, by counting: of the values that fewer than num are above, the
 // smallest.  `all` has a place for every thread.
-template <typename T>
-__device__ inline T reached_by(T mine, int num, T largest_possible, T* all) {
+__device__ inline float reached_by(float mine, int num, float* all) {
   all[threadIdx.x] = mine;
   __syncthreads();
   int above = 0;
 #pragma unroll 8
   for (int i = 0; i < kThreads; ++i) above += all[i] > mine;
-  T least = above < num ? mine : largest_possible;
+  float least = above < num ? mine : INFINITY;
   for (int step = 32; step > 0; step >>= 1) {
-    const T other = __shfl_xor(least, step);
-    least = other < least ? other : least;
+    least = fminf(least, __shfl_xor(least, step));
   }
   __syncthreads();
   if ((threadIdx.x & 63) == 0) all[threadIdx.x >> 6] = least;
   __syncthreads();
-  for (int w = 0; w < kWaves; ++w) least = all[w] < least ? all[w] : least;
+  for (int w = 0; w < kWaves; ++w) least = fminf(least, all[w]);
   return least;
 }
 
@@ -191,16 +190,17 @@ __global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) 
             sum *= __builtin_amdgcn_exp2f((top - largest) * kLog2e);
             top = largest;
           }
-          const float base = top == -INFINITY ? 0.f : top, before = sum;
-          if (t == 0) sum += __builtin_amdgcn_exp2f((extra - base) * kLog2e);
+          const float base = top == -INFINITY ? 0.f : top;
+          float of_tile = t == 0 ? __builtin_amdgcn_exp2f((extra - base) * kLog2e) : 0.f;
 #pragma unroll
-          for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);
+          for (int i = 0; i < EACH; ++i) of_tile += __builtin_amdgcn_exp2f((v[i] - base) * kLog2e);
           if (top == INFINITY) {  // (beside an infinite one only the infinite ones count)
-            sum = before + (t == 0 && extra == INFINITY ? 1.f : 0.f);
-            for (int i = 0; i < EACH; ++i) sum += v[i] == INFINITY ? 1.f : 0.f;
+            of_tile = t == 0 && extra == INFINITY ? 1.f : 0.f;
+            for (int i = 0; i < EACH; ++i) of_tile += v[i] == INFINITY ? 1.f : 0.f;
           }
+          sum += of_tile;
         }
-        if (t == 0) bar = fmaxf(reached_by(largest, a.most, INFINITY, shared), kLowest);
+        if (t == 0) bar = fmaxf(reached_by(largest, a.most, shared), kLowest);
       }
       auto offer = [&](float value, int at_row) {
         const bool in = value >= bar;
@@ -267,125 +267,187 @@ __device__ inline double total_value(uint64_t u) {
   return __longlong_as_double((long long)(u & 0x8000000000000000ull ? u & 0x7fffffffffffffffull : ~u));
 }
 
-// The lists of a batch entry's beams and parts become its answer: the totals in 64 bits, those that num of the threads' best
-// reach in LDS, each ranked among them by (total, lower beam, its own order).
-__global__ void __launch_bounds__(kThreads) select_merge_kernel(SelectArgs a) {
+// The lists of a batch entry's beams and parts become its answer: the totals in 64 bits, all of them in registers; a bar that at
+// least num of them reach and not many more; those in LDS, each ranked there by (total, lower beam, its own order).  Four lanes
+// count for one value.  One workgroup for each batch entry, and what it does is a chain of short steps: its waits are its time.
+constexpr int kMerge = 1024, kMergeWaves = kMerge / 64, kGroups = kMerge / 4;
+
+// HELD: candidates of a thread.  Few ones' code is a third of the other's, and it is read from memory at every call: what it saved
+// is beside the plan.
+template <int HELD>
+__global__ void __launch_bounds__(kMerge) select_merge_kernel(SelectArgs a) {
   __shared__ uint64_t kept_total[kKept], kept_key[kKept];
   __shared__ int kept_beam[kKept];
-  __shared__ uint64_t shared[kThreads];
+  __shared__ uint64_t group_best[kGroups];
+  __shared__ int counts[2][kMergeWaves];
   __shared__ int filled, first_best;
-  extern __shared__ double beam_less[];  // per beam: the logarithm of its sum, and its largest score behind
-  double* beam_top = beam_less + a.num_beams;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  extern __shared__ double beam_less[];  // per beam: the logarithm of its sum, its largest score (NaN: finished), what it gathered
+  float* beam_top = reinterpret_cast<float*>(beam_less + a.num_beams);
+  float* beam_has = beam_top + a.num_beams;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per_beam = a.parts * a.most, all = a.num_beams * per_beam;
-  for (int k = tid >> 6; a.normalise && k < a.num_beams; k += kWaves) {
+  const uint64_t* lists = a.lists + (long long)b * all;
+  for (int k = wave; k < a.num_beams; k += kMergeWaves) {
     const long long row = (long long)b * a.num_beams + k;
-    if (a.finished && a.finished[row]) continue;
-    float top = -INFINITY;
-    for (int p = lane; p < a.parts; p += 64) top = fmaxf(top, a.list_top[row * a.parts + p]);
-    for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
-    double sum = 0.0;
-    for (int p = lane; p < a.parts; p += 64) {
-      const float t = a.list_top[row * a.parts + p];
-      const double s = a.list_sum[row * a.parts + p];
-      if (t > -INFINITY) sum += t == top ? s : s * exp((double)t - (double)top);
+    const bool done = a.finished && a.finished[row];
+    const float has = a.beams ? a.beams[row] : 0.f;
+    float top = done ? NAN : 0.f;
+    double sum = 1.0;
+    if (a.normalise && !done) {
+      const float first_top = lane < a.parts ? a.list_top[row * a.parts + lane] : -INFINITY;
+      const double first_sum = lane < a.parts ? a.list_sum[row * a.parts + lane] : 0.0;
+      top = first_top;
+      for (int p = lane + 64; p < a.parts; p += 64) top = fmaxf(top, a.list_top[row * a.parts + p]);
+      for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
+      sum = 0.0;
+      for (int p = lane; p < a.parts; p += 64) {
+        const float t = p < 64 ? first_top : a.list_top[row * a.parts + p];
+        const double s = p < 64 ? first_sum : a.list_sum[row * a.parts + p];
+        if (t > -INFINITY) sum += t == top ? s : s * exp((double)t - (double)top);
+      }
+      for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
     }
-    for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
     if (lane == 0) {
       beam_top[k] = top;
-      beam_less[k] = log(sum);
+      beam_has[k] = has;
+      beam_less[k] = a.normalise ? log(sum) : 0.0;
     }
   }
   if (tid == 0) filled = 0;
+  uint64_t totals[HELD];  // 0: no candidate
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) totals[i] = tid + i * kMerge < all ? lists[tid + i * kMerge] : 0;
   __syncthreads();
-  auto key_of = [&](int c) { return a.lists[(long long)b * all + c]; };
-  auto total_of = [&](int c, uint64_t key) -> uint64_t {  // 0: no candidate
-    const int k = c / per_beam;
-    const long long row = (long long)b * a.num_beams + k;
-    const double beam = a.beams ? a.beams[row] : 0.f;
-    double total;
-    if (a.finished && a.finished[row]) {
-      if (c != k * per_beam) return 0;
-      total = beam;
-    } else {
-      if (key == 0) return 0;
-      total = key_value(key);
-      if (a.normalise) total = (total == beam_top[k] ? 0.0 : total - beam_top[k]) - beam_less[k];
-      total += beam;
+  uint64_t best = 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    if (i * kMerge >= all) continue;
+    const int c = tid + i * kMerge, k = c / per_beam;
+    const uint64_t key = totals[i];
+    totals[i] = 0;
+    if (c < all) {
+      const double has = beam_has[k], top = beam_top[k];
+      double total = -INFINITY;
+      if (top != top) {
+        if (c == k * per_beam) total = has;
+      } else if (key != 0) {
+        total = key_value(key);
+        total = (total == top ? 0.0 : total - top) - beam_less[k] + has;
+      }
+      if (total > -INFINITY) totals[i] = order_total(total);
     }
-    return total > -INFINITY ? order_total(total) : 0;
-  };
-  constexpr int kHeld = 4;  // candidates of a thread that stay in registers
-  uint64_t best = 0, keys[kHeld], totals[kHeld];
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) keys[i] = tid + i * kThreads < all ? key_of(tid + i * kThreads) : 0;
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    totals[i] = tid + i * kThreads < all ? total_of(tid + i * kThreads, keys[i]) : 0;
     best = totals[i] > best ? totals[i] : best;
   }
-  for (int c = tid + kHeld * kThreads; c < all; c += kThreads) {
-    const uint64_t t = total_of(c, key_of(c));
-    best = t > best ? t : best;
+  auto key_of = [&](int c, int k) -> uint64_t { return beam_top[k] != beam_top[k] ? (uint64_t)(uint32_t)~(uint32_t)a.end : lists[c]; };
+
+  // The num-th largest of the groups' best: of those that fewer than num are above, the smallest.
+  for (int step = 1; step < 4; step <<= 1) {
+    const uint64_t other = __shfl_xor(best, step);
+    best = other > best ? other : best;
   }
-  const uint64_t bar = reached_by(best, a.num, ~(uint64_t)0, shared);
-  auto offer = [&](int c, uint64_t key, uint64_t t) {
-    if (t == 0 || t < bar) return;
-    const int at = atomicAdd(&filled, 1);
-    if (at >= kKept) return;
-    const int k = c / per_beam;
-    kept_total[at] = t;
-    kept_key[at] = a.finished && a.finished[(long long)b * a.num_beams + k] ? (uint64_t)(uint32_t)~(uint32_t)a.end : key;
-    kept_beam[at] = k;
-  };
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) offer(tid + i * kThreads, keys[i], totals[i]);
-  if (best >= bar)
-    for (int c = tid + kHeld * kThreads; c < all; c += kThreads) {
-      const uint64_t key = key_of(c);
-      offer(c, key, total_of(c, key));
-    }
+  if ((lane & 3) == 0) group_best[tid >> 2] = best;
   __syncthreads();
-  const int count = filled;
+  uint64_t bar, beyond = best;
+  {
+    int above = 0;
+#pragma unroll 8
+    for (int i = lane & 3; i < kGroups; i += 4) above += group_best[i] > best;
+    above += __shfl_xor(above, 1);
+    above += __shfl_xor(above, 2);
+    bar = above < a.num ? best : ~(uint64_t)0;
+    for (int step = 32; step > 0; step >>= 1) {
+      const uint64_t low = __shfl_xor(bar, step), high = __shfl_xor(beyond, step);
+      bar = low < bar ? low : bar;
+      beyond = high > beyond ? high : beyond;
+    }
+    if (lane == 0) kept_total[wave] = bar, kept_key[wave] = beyond;
+    __syncthreads();
+    for (int w = 0; w < kMergeWaves; ++w) {
+      bar = kept_total[w] < bar ? kept_total[w] : bar;
+      beyond = kept_key[w] > beyond ? kept_key[w] : beyond;
+    }
+    beyond += 1;
+  }
+  if (bar == 0) bar = 1;
+  // How many reach the bar: while they are many more than asked for, and not all equal, it is raised by halving.
+  const int enough = a.num + kGroups;
+  int count = 0;
+  uint64_t probe = bar;
+  for (int turn = 0;; turn ^= 1) {
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (i * kMerge < all) reach += __popcll(__ballot(totals[i] >= probe));
+    if (lane == 0) counts[turn][wave] = reach;
+    __syncthreads();
+    reach = 0;
+    for (int w = 0; w < kMergeWaves; ++w) reach += counts[turn][w];
+    if (probe == bar || reach >= a.num) {
+      bar = probe;
+      count = reach;
+    } else {
+      beyond = probe;
+    }
+    if (count <= enough || beyond - bar <= 1) break;
+    probe = bar + (beyond - bar) / 2;
+  }
   const long long out = (long long)b * a.num;
-  if (count <= kKept) {
-    for (int i = tid; i < count; i += kThreads) {
-      const uint64_t t = kept_total[i], key = kept_key[i];
-      const int k = kept_beam[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < count; ++j) {
-        const uint64_t other = kept_total[j];
-        if (other == t) rank += kept_beam[j] < k || (kept_beam[j] == k && kept_key[j] > key);
-        else rank += other > t;
+  int divisor = per_beam;  // (hidden, so that the quotients are worked out again where they are used and not kept in registers)
+  asm volatile("" : "+s"(divisor));
+  if (HELD * kMerge <= kKept || count <= kKept) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (totals[i] >= bar) {
+        const int at = atomicAdd(&filled, 1), c = tid + i * kMerge, k = c / divisor;
+        kept_total[at] = totals[i];
+        kept_key[at] = key_of(c, k);
+        kept_beam[at] = k;
       }
-      if (rank < a.num) {
+    __syncthreads();
+    for (int first = 0; first < count; first += kGroups) {
+      const int i = first + (tid >> 2);
+      int rank = 0;
+      uint64_t t = 0, key = 0;
+      int k = 0;
+      if (i < count) {
+        t = kept_total[i], key = kept_key[i], k = kept_beam[i];
+#pragma unroll 4
+        for (int j = lane & 3; j < count; j += 4) {
+          const uint64_t other = kept_total[j];
+          if (other == t) rank += kept_beam[j] < k || (kept_beam[j] == k && kept_key[j] > key);
+          else rank += other > t;
+        }
+      }
+      rank += __shfl_xor(rank, 1);
+      rank += __shfl_xor(rank, 2);
+      if (i < count && (lane & 3) == 0 && rank < a.num) {
         a.out_totals[out + rank] = (float)total_value(t);
         a.out_parents[out + rank] = k;
         a.out_tokens[out + rank] = key_place(key);
       }
     }
-    for (int i = count + tid; i < a.num; i += kThreads) {
+    for (int i = count + tid; i < a.num; i += kMerge) {
       a.out_totals[out + i] = -INFINITY;
       a.out_parents[out + i] = a.out_tokens[out + i] = -1;
     }
     return;
   }
-  // More equal totals than are held: one after the other, each the best of those behind the last one.
+  // More equal totals than are held (of more candidates than are held): one after the other, each the best of those behind the last one.
   uint64_t last = ~0ull, last_key = 0;
   int last_beam = -1;
-  for (int i = 0; i < a.num; ++i) {
+  auto before = [](uint64_t t, int k, uint64_t key, uint64_t t2, int k2, uint64_t key2) {
+    return t != t2 ? t > t2 : k != k2 ? k < k2 : key > key2;
+  };
+  for (int n = 0; n < a.num; ++n) {
     uint64_t mine = 0, mine_key = 0;
     int mine_beam = 0;
-    auto before = [](uint64_t t, int k, uint64_t key, uint64_t t2, int k2, uint64_t key2) {
-      return t != t2 ? t > t2 : k != k2 ? k < k2 : key > key2;
-    };
-    for (int c = tid; c < all; c += kThreads) {
-      const int k = c / per_beam;
-      uint64_t key = key_of(c);
-      const uint64_t t = total_of(c, key);
-      if (t == 0) continue;
-      if (a.finished && a.finished[(long long)b * a.num_beams + k]) key = (uint64_t)(uint32_t)~(uint32_t)a.end;
+    asm volatile("" : "+s"(divisor));
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      const uint64_t t = totals[i];
+      if (t < bar) continue;
+      const int c = tid + i * kMerge, k = c / divisor;
+      const uint64_t key = key_of(c, k);
       if (last_beam >= 0 && !before(last, last_beam, last_key, t, k, key)) continue;
       if (mine == 0 || before(t, k, key, mine, mine_beam, mine_key)) mine = t, mine_key = key, mine_beam = k;
     }
@@ -395,29 +457,21 @@ __global__ void __launch_bounds__(kThreads) select_merge_kernel(SelectArgs a) {
       if (t != 0 && (mine == 0 || before(t, k, key, mine, mine_beam, mine_key))) mine = t, mine_key = key, mine_beam = k;
     }
     __syncthreads();
-    if (lane == 0) kept_total[tid >> 6] = mine, kept_key[tid >> 6] = mine_key, kept_beam[tid >> 6] = mine_beam;
+    if (lane == 0) kept_total[wave] = mine, kept_key[wave] = mine_key, kept_beam[wave] = mine_beam;
     __syncthreads();
-    if (tid == 0) {
+    if (tid == 0) {  // (there are num of them: more than are held reach the bar)
       int w = 0;
-      for (int o = 1; o < kWaves; ++o)
+      for (int o = 1; o < kMergeWaves; ++o)
         if (kept_total[o] != 0 && (kept_total[w] == 0 || before(kept_total[o], kept_beam[o], kept_key[o], kept_total[w], kept_beam[w], kept_key[w]))) w = o;
       first_best = w;
-      const bool there = kept_total[w] != 0;
-      a.out_totals[out + i] = there ? (float)total_value(kept_total[w]) : -INFINITY;
-      a.out_parents[out + i] = there ? kept_beam[w] : -1;
-      a.out_tokens[out + i] = there ? key_place(kept_key[w]) : -1;
+      a.out_totals[out + n] = (float)total_value(kept_total[w]);
+      a.out_parents[out + n] = kept_beam[w];
+      a.out_tokens[out + n] = key_place(kept_key[w]);
     }
     __syncthreads();
     last = kept_total[first_best];
     last_key = kept_key[first_best];
     last_beam = kept_beam[first_best];
-    if (last == 0) {  // (nothing is left)
-      for (int j = i + 1 + tid; j < a.num; j += kThreads) {
-        a.out_totals[out + j] = -INFINITY;
-        a.out_parents[out + j] = a.out_tokens[out + j] = -1;
-      }
-      return;
-    }
   }
 }
 
@@ -482,7 +536,7 @@ static SelectPlan select_plan(int type, int num_batch, int num_beams, int num_va
   p.small = rows * num_values < 512ll * 8192;
   const long long tile = kThreads * (p.small ? 16 / (long long)element_size(type) : 16);
   const int tiles = (int)((num_values + tile - 1) / tile);
-  const long long wanted = std::min<long long>({std::max<long long>(1, kResident / rows), 256, std::max<long long>(1, 16384 / ((long long)num_beams * most))});
+  const long long wanted = std::min<long long>({std::max<long long>(1, kResident / rows), 256, std::max<long long>(1, kMostCandidates / ((long long)num_beams * most))});
   p.each = (int)((tiles + wanted - 1) / wanted);
   p.parts = (tiles + p.each - 1) / p.each;
   return p;
@@ -544,7 +598,9 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
       else if (normalise) hipLaunchKernelGGL((select_part_kernel<T, sizeof(T), true>), grid, dim3(kThreads), 0, s, a);
       else hipLaunchKernelGGL((select_part_kernel<T, sizeof(T), false>), grid, dim3(kThreads), 0, s, a);
     });
-    hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)num_batch), dim3(kThreads), (size_t)num_beams * 16, s, a);
+    const int candidates = num_beams * p.parts * a.most;
+    if (candidates <= 2 * kMerge) hipLaunchKernelGGL(select_merge_kernel<2>, dim3((unsigned)num_batch), dim3(kMerge), (size_t)num_beams * 16, s, a);
+    else hipLaunchKernelGGL(select_merge_kernel<kMostCandidates / kMerge>, dim3((unsigned)num_batch), dim3(kMerge), (size_t)num_beams * 16, s, a);
     HIP_CHECK(hipGetLastError());
   });
 }

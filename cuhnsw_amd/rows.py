@@ -336,7 +336,10 @@ def select_beams(scores, beams, num, normalise=True, finished=None, end=None):
   None (zeros).  A candidate's total is beams + scores, with normalise beams + log_softmax(scores); totals are compared in 64
   bits, equal ones go to the lower beam, then the larger score, then the lower token.  Masked places hold -infinity (a NaN counts as
   one): they are never chosen, and where too few candidates are left the rest says -infinity, -1, -1.  finished: bool
-  [batch, beams] or None: a finished beam has one candidate, token `end`, with what it gathered."""
+  [batch, beams] or None: a finished beam has one candidate, token `end`, with what it gathered.
+
+  The same call gives the same answer to the last bit; how a row's sum of exponentials is split depends on the sizes, so that
+  a row's totals can differ in their last bits between batches of different sizes."""
   _tensor(scores, "scores", 3)
   _check(isinstance(num, int) and 0 < num <= 256, "num is between 1 and 256")
   b, k, v = scores.shape
