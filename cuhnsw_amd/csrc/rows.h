@@ -34,9 +34,7 @@ template <>
 __device__ inline _Float16 narrow<_Float16>(float x) { return (_Float16)x; }
 template <>
 __device__ inline bf16 narrow<bf16>(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const uint32_t rounded = (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-  return bf16{(uint16_t)((u & 0x7fffffffu) > 0x7f800000u ? (u >> 16) | 0x40u : rounded)};
+  return bf16{__builtin_bit_cast(uint16_t, (__bf16)x)};  // (one instruction of the machine)
 }
 
 // n elements that move together (the widest such access that rows, strides and addresses allow is chosen per call)

@@ -91,6 +91,8 @@ constexpr int kTile = 16, kUnit = 32, kRowTiles = 4;  // queries or rows of a ma
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bfloat2_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 
 struct ScoresArgs {
@@ -257,12 +259,12 @@ __device__ inline void exchange(uint4 words, uint32_t (&slots)[4]) {
 __device__ inline void transpose_quad(uint32_t (&x)[4]) {
   const int l = threadIdx.x & 3;
   auto swap = [&](uint32_t& low, uint32_t& high, bool upper, auto dpp) {
-    const uint32_t mine = upper ? low : high, theirs = dpp(mine);
-    low = upper ? theirs : low;
-    high = upper ? high : theirs;
+    const uint32_t their_low = dpp(low), their_high = dpp(high);
+    low = upper ? their_high : low;
+    high = upper ? high : their_low;
   };
-  auto next = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true); };     // lanes 1 0 3 2
-  auto over = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true); };     // lanes 2 3 0 1
+  auto next = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, true); };     // lanes 1 0 3 2
+  auto over = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, true); };     // lanes 2 3 0 1
   swap(x[0], x[1], l & 1, next);
   swap(x[2], x[3], l & 1, next);
   swap(x[0], x[2], l & 2, over);
@@ -279,7 +281,7 @@ __device__ inline void store_scores(const ScoresArgs& a, const float4_t (&acc)[R
   const long long first = row - l * RT;  // of the four lanes' rows
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    auto score = [&](int r, int t) { return a.alpha * ldexpf(acc[t][m][r], (signed char)(exponents[m] >> (8 * r))) + bias[t]; };
+    auto score = [&](int r, int t) { return fmaf(a.alpha, ldexpf(acc[t][m][r], (signed char)(exponents[m] >> (8 * r))), bias[t]); };
     if (a.out_type == TYPE_F32) {
       const int rows = (int)max(0ll, min((long long)RT, a.num_rows - row));
 #pragma unroll
@@ -308,8 +310,8 @@ __device__ inline void store_scores(const ScoresArgs& a, const float4_t (&acc)[R
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float low = score(r, 2 * w), high = score(r, 2 * w + 1);
-          words[w][r] = a.out_type == TYPE_BF16 ? narrow<bf16>(low).bits | (uint32_t)narrow<bf16>(high).bits << 16
-                                                : __builtin_bit_cast(uint16_t, (_Float16)low) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)high) << 16;
+          words[w][r] = a.out_type == TYPE_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{low, high}), bfloat2_t))
+                                                : __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{low, high}), half2_t));
         }
         transpose_quad(words[w]);
       }
