@@ -117,59 +117,82 @@ struct ScoresArgs {
   int query_blocks, row_blocks, split, blocks_each;
 };
 
-// Power of two that takes the largest magnitude of a query to [2^14, 2^15): the exponent of the largest element, by the whole
-// workgroup.  A float16 query stays as it is, and one that is zero or not finite too.
+// Eight elements of a query, 0 behind the last one.
 template <typename T>
-__device__ inline int exponent_of(const T* q, int num_dims, float* per_wave) {
-  if (std::is_same_v<T, _Float16>) return 14;
-  const int tid = threadIdx.x, threads = blockDim.x;
-  float most = 0.f;
-  for (int k = tid; k < num_dims; k += threads) {
-    const float x = fabsf(widen(q[k]));
-    most = x < INFINITY ? fmaxf(most, x) : INFINITY;  // (a NaN too)
-  }
-  for (int step = 32; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
-  if ((tid & 63) == 0) per_wave[tid >> 6] = most;
-  __syncthreads();
-  for (int w = 0; w < threads / 64; ++w) most = fmaxf(most, per_wave[w]);
-  __syncthreads();
-  return most > 0.f && most < INFINITY ? max(ilogbf(most), -126) : 14;  // (a byte holds it)
-}
-// Eight elements, a quarter of a unit, in the order in which the codes of a word come apart: 0 4 1 5 2 6 3 7.
-template <typename T>
-__device__ inline void planes_of_eight(const T* q, int first, int num_dims, int exponent, half8_t& high, half8_t& low) {
+__device__ inline LoosePack<T, 8> eight_of(const T* q, int first, int num_dims) {
+  LoosePack<T, 8> x;
+  if (first + 8 <= num_dims) {
+    x = *reinterpret_cast<const LoosePack<T, 8>*>(q + first);
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int k = first + (e & 1) * 4 + (e >> 1);
-    const float x = k < num_dims ? ldexpf(widen(q[k]), 14 - exponent) : 0.f;
-    high[e] = (_Float16)x;
-    low[e] = (_Float16)(x - (float)high[e]);
+    for (int e = 0; e < 8; ++e) x.at[e] = first + e < num_dims ? q[first + e] : narrow<T>(0.f);
   }
+  return x;
 }
-template <typename T>
-__device__ inline float sum_of_group(const T* q, int g, const ScoresArgs& a, int exponent) {
-  float sum = 0.f;
-  for (int k = g * a.group; k < min(a.num_dims, (g + 1) * a.group); ++k) sum += ldexpf(widen(q[k]), -exponent);
-  return sum;
+
+// A workgroup lays a query out.  A power of two takes its largest magnitude to [2^14, 2^15) (a float16 query stays as it is, and
+// one that is zero or not finite too): returned is the exponent of the largest element.  put(w, high, low) gets the planes of elements
+// 8 w to 8 w + 7, in the order in which the codes of a word come apart (0 4 1 5 2 6 3 7), put_sum(g, sum) the sums of the
+// groups if `with_sums`.
+template <typename T, typename Put, typename PutSum>
+__device__ inline int lay_out(const T* q, int num_dims, int pieces, int group, int groups, bool with_sums, float* per_wave, Put put, PutSum put_sum) {
+  const int tid = threadIdx.x, threads = blockDim.x, lanes = group / 8;
+  const LoosePack<T, 8> held = eight_of(q, tid * 8, num_dims);
+  int exponent = 14;
+  if (!std::is_same_v<T, _Float16>) {
+    float most = 0.f;
+    auto look_at = [&](const LoosePack<T, 8>& x) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = fabsf(widen(x.at[e]));
+        most = y < INFINITY ? fmaxf(most, y) : INFINITY;  // (a NaN too)
+      }
+    };
+    look_at(held);
+    for (int w = tid + threads; w * 8 < num_dims; w += threads) look_at(eight_of(q, w * 8, num_dims));
+    for (int step = 32; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor(most, step));
+    if ((tid & 63) == 0) per_wave[tid >> 6] = most;
+    __syncthreads();
+    for (int w = 0; w < threads / 64; ++w) most = fmaxf(most, per_wave[w]);
+    __syncthreads();
+    if (most > 0.f && most < INFINITY) exponent = max(ilogbf(most), -126);  // (a byte holds it)
+  }
+  for (int first = 0; first < pieces; first += threads) {  // (lanes of one group come this way together)
+    const int w = first + tid;
+    const LoosePack<T, 8> x = first == 0 ? held : eight_of(q, w * 8, num_dims);
+    half8_t high, low;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = ldexpf(widen(x.at[(e & 1) * 4 + (e >> 1)]), 14 - exponent);
+      high[e] = (_Float16)y;
+      low[e] = (_Float16)(y - (float)high[e]);
+      sum += ldexpf(y, -14);
+    }
+    if (w < pieces) put(w, high, low);
+    if (with_sums) {
+      for (int step = 1; step < lanes; step <<= 1) sum += __shfl_xor(sum, step);
+      if (w % lanes == 0 && w / lanes < groups) put_sum(w / lanes, sum);
+    }
+  }
+  return exponent;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) prepare_kernel(ScoresArgs a, int planes) {
   __shared__ float per_wave[4];
-  const int m = blockIdx.x, tid = threadIdx.x, tile = m / kTile, i = m % kTile;
+  const int m = blockIdx.x, tile = m / kTile, i = m % kTile;
   const bool there = m < a.num_queries;  // (the last tile is filled up with zeros)
   const T* q = static_cast<const T*>(a.queries) + (there ? m : 0) * a.query_stride;
-  const int num_dims = there ? a.num_dims : 0, exponent = exponent_of(q, num_dims, per_wave);
-  if (tid == 0) a.exponents[m] = (signed char)exponent;
   _Float16* to = a.planes + (size_t)tile * kTile * a.padded_units * kUnit;
-  for (int w = tid; w < a.padded_units * 4; w += 256) {
-    half8_t high, low;
-    planes_of_eight(q, w * 8, num_dims, exponent, high, low);
-    *reinterpret_cast<half8_t*>(to + ((size_t)w * kTile + i) * 8) = high;
-    if (planes == 2) *reinterpret_cast<half8_t*>(to + a.plane + ((size_t)w * kTile + i) * 8) = low;
-  }
-  if (a.offsets)
-    for (int g = tid; g < a.groups; g += 256) a.sums[((size_t)tile * a.groups + g) * kTile + i] = there ? sum_of_group(q, g, a, exponent) : 0.f;
+  const int exponent = lay_out(
+      q, there ? a.num_dims : 0, a.padded_units * 4, a.group, a.groups, a.offsets != nullptr, per_wave,
+      [&](int w, half8_t high, half8_t low) {
+        *reinterpret_cast<half8_t*>(to + ((size_t)w * kTile + i) * 8) = high;
+        if (planes == 2) *reinterpret_cast<half8_t*>(to + a.plane + ((size_t)w * kTile + i) * 8) = low;
+      },
+      [&](int g, float sum) { a.sums[((size_t)tile * a.groups + g) * kTile + i] = sum; });
+  if (threadIdx.x == 0) a.exponents[m] = (signed char)exponent;
 }
 
 // The eight codes of a word, less 8 or as they are, as float16, in the order 0 4 1 5 2 6 3 7: a code behind the exponent of 1024
@@ -402,16 +425,14 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
   if (OWN) {
     for (int i = 0; i < own_queries; ++i) {
       const T* q = static_cast<const T*>(a.queries) + i * a.query_stride;
-      const int exponent = exponent_of(q, a.num_dims, per_wave);
+      const int exponent = lay_out(
+          q, a.num_dims, a.padded_units * 4, a.group, a.groups, !CENTRED, per_wave,
+          [&](int w, half8_t high, half8_t low) {
+            *reinterpret_cast<half8_t*>(own + ((size_t)w * own_queries + i) * 8) = high;
+            if (PLANES == 2) *reinterpret_cast<half8_t*>(own + own_plane + ((size_t)w * own_queries + i) * 8) = low;
+          },
+          [&](int g, float sum) { own_sums[g * kTile + i] = sum; });
       if (threadIdx.x == 0) own_exponents[i] = (signed char)exponent;
-      for (int w = threadIdx.x; w < a.padded_units * 4; w += blockDim.x) {
-        half8_t high, low;
-        planes_of_eight(q, w * 8, a.num_dims, exponent, high, low);
-        *reinterpret_cast<half8_t*>(own + ((size_t)w * own_queries + i) * 8) = high;
-        if (PLANES == 2) *reinterpret_cast<half8_t*>(own + own_plane + ((size_t)w * own_queries + i) * 8) = low;
-      }
-      if (!CENTRED)
-        for (int g = threadIdx.x; g < a.groups; g += blockDim.x) own_sums[g * kTile + i] = sum_of_group(q, g, a, exponent);
     }
     __syncthreads();
   }
