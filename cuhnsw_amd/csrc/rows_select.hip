@@ -17,7 +17,7 @@ namespace cuhnsw_amd {
 
 constexpr int kMostNum = 256, kMostBeams = 1024, kMostLists = 4096;
 constexpr int kMostCandidates = 16384;  // in the lists of a batch entry: what one workgroup holds in registers
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256, kWaves = 4, kEach = 16;
 constexpr int kKept = 2048;  // candidates a workgroup holds in LDS
 
 struct SelectArgs {
@@ -68,65 +68,81 @@ __device__ inline float reached_by(float mine, int num, float* all) {
 }
 
 // The best of `count` different keys to the front, in order; how many there are then (at most `most`).  Up to two for every thread are
-// ranked by counting the larger ones, more go through a bitonic network.
-__device__ inline int keep_best(uint64_t* keys, int count, int most) {
-  const int tid = threadIdx.x;
+// ranked by counting the larger ones.  Of more (up to kKept) those are picked first that reach a bar which enough of them
+// reach and no more than that: it is found by halving, with the keys in registers.
+__device__ inline int keep_best(uint64_t* keys, int count, int most, int (&counts)[2][kWaves]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __syncthreads();
-  if (count <= 2 * kThreads) {
-    uint64_t mine[2];
-    int rank[2] = {0, 0};
-    for (int j = 0; j < 2; ++j) mine[j] = tid + j * kThreads < count ? keys[tid + j * kThreads] : 0;
-    if (count <= kThreads) {
-#pragma unroll 8
-      for (int i = 0; i < count; ++i) rank[0] += keys[i] > mine[0];
-    } else {
-#pragma unroll 8
-      for (int i = 0; i < count; ++i) {
-        const uint64_t other = keys[i];
-        rank[0] += other > mine[0];
-        rank[1] += other > mine[1];
+  if (count > 2 * kThreads) {
+    constexpr int kMine = kKept / kThreads;
+    uint64_t mine[kMine], bar = 1, beyond = ~0ull;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) mine[i] = tid + i * kThreads < count ? keys[tid + i * kThreads] : 0;
+    int turn = 0, before;
+    for (uint64_t probe = beyond / 2;; probe = bar + (beyond - bar) / 2, turn ^= 1) {
+      int reach = 0;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) reach += __popcll(__ballot(mine[i] >= probe));
+      if (lane == 0) counts[turn][wave] = reach;
+      __syncthreads();
+      reach = before = 0;
+      for (int w = 0; w < kWaves; ++w) {
+        before += w < wave ? counts[turn][w] : 0;
+        reach += counts[turn][w];
+      }
+      if (reach < most) {
+        beyond = probe;
+      } else {
+        bar = probe;
+        count = reach;
+        if (count <= 2 * kThreads) break;
       }
     }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const unsigned long long with = __ballot(mine[i] >= bar);
+      if (mine[i] >= bar) keys[before + __popcll(with & ((1ull << lane) - 1))] = mine[i];
+      before += __popcll(with);
+    }
     __syncthreads();
-    for (int j = 0; j < 2; ++j)
-      if (mine[j] && rank[j] < most) keys[rank[j]] = mine[j];
-  } else {
-    int size = 1024;
-    while (size < count) size <<= 1;
-    for (int i = count + tid; i < size; i += kThreads) keys[i] = 0;
-    for (int run = 2; run <= size; run <<= 1)
-      for (int step = run >> 1; step > 0; step >>= 1) {
-        __syncthreads();
-        for (int i = tid; i < size / 2; i += kThreads) {
-          const int a = (i / step) * 2 * step + i % step, b = a + step;
-          const uint64_t x = keys[a], y = keys[b];
-          if ((x < y) == ((a & run) == 0)) {
-            keys[a] = y;
-            keys[b] = x;
-          }
-        }
-      }
   }
+  uint64_t mine[2];
+  int rank[2] = {0, 0};
+  for (int j = 0; j < 2; ++j) mine[j] = tid + j * kThreads < count ? keys[tid + j * kThreads] : 0;
+  if (count <= kThreads) {
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) rank[0] += keys[i] > mine[0];
+  } else {
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      const uint64_t other = keys[i];
+      rank[0] += other > mine[0];
+      rank[1] += other > mine[1];
+    }
+  }
+  __syncthreads();
+  for (int j = 0; j < 2; ++j)
+    if (mine[j] && rank[j] < most) keys[rank[j]] = mine[j];
   __syncthreads();
   return min(count, most);
 }
 
-// Pass over a row's scores: NV vectors of 16 bytes for each thread are a tile, and the next tile is asked for before the one
-// at hand is looked at.  The first tile gives a value that `num` of its scores reach; a score that is not below it goes to a list in
+// Pass over a row's scores: 16 for each thread are a tile, in vectors of 16 bytes, and the next tile is asked for before the
+// one at hand is looked at.  The first tile gives a value that `num` of its scores reach; a score that is not below it goes to a list in
 // LDS.  After 1, 2, 4, 8... tiles the list is cut down to its best, and what comes later has to reach the worst of them: a hundred
 // or so enter between two cuts, and between two cuts the wavefronts do not wait for each other.  Where a list would
 // overflow meanwhile (scores in an order that is hard) those tiles are gone over again, a score of each thread at a time.
 //
 // What a score costs: its conversion, a comparison, and normalised the maximum, a subtraction, a product, the exponential (of four
 // times the cost) and an addition.
-template <typename T, int NV, bool NORMALISE>
+template <typename T, bool NORMALISE>
 __global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) {
-  constexpr int VE = 16 / sizeof(T), EACH = NV * VE;
+  constexpr int VE = 16 / sizeof(T), EACH = kEach, NV = EACH / VE;
   typedef LoosePack<T, VE> Vector;
   __shared__ uint64_t kept[kKept];
   __shared__ float shared[kThreads];
   __shared__ double shared_sum[kWaves];
-  __shared__ int filled;
+  __shared__ int filled, counts[2][kWaves];
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, b = row / a.num_beams, k = row - b * a.num_beams;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (a.finished && a.finished[row]) return;
@@ -157,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) 
   float bar = 0.f;       // what a score has to reach (always finite: -infinity and NaN never do)
   constexpr float kLowest = -3.402823466e38f;
   auto cut = [&] {
-    have = keep_best(kept, have, a.most);
+    have = keep_best(kept, have, a.most, counts);
     if (have == a.most) {
       bar_key = kept[have - 1];
       bar = fmaxf(key_value(bar_key), kLowest);
@@ -236,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 6) select_part_kernel(SelectArgs a) 
     if (t < tiles && have > a.most) cut();
     __syncthreads();
   }
-  have = keep_best(kept, have, a.most);
+  have = keep_best(kept, have, a.most, counts);
   uint64_t* list = a.lists + (long long)blockIdx.x * a.most;
   for (int i = tid; i < a.most; i += kThreads) list[i] = i < have ? kept[i] : 0;
   if (NORMALISE) {
@@ -522,22 +538,19 @@ __global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a) {
   }
 }
 
-// How a selection is spread: tiles of one vector or of 16 scores for each thread, and so many workgroups a row as the machine
-// holds at once (six on a CU: one more would be a second round).
-constexpr int kResident = 6 * 256;
+// How a selection is spread: as many workgroups a row as the machine holds at once (six on a CU: one more would be a second round)
+// and as the last step can hold candidates of.  Of a row of 1 000 000 float32 scores (the best ten) 16, 64 and 256
+// workgroups take 30, 22 and 19 us.
+constexpr int kResident = 6 * 256, kMostParts = 256;
 struct SelectPlan {
-  bool small;
   int parts, each;
 };
-static SelectPlan select_plan(int type, int num_batch, int num_beams, int num_values, int num) {
-  SelectPlan p;
+static SelectPlan select_plan(int num_batch, int num_beams, int num_values, int num) {
   const long long rows = (long long)num_batch * num_beams;
-  const int most = std::min(num, num_values);
-  p.small = rows * num_values < 512ll * 8192;
-  const long long tile = kThreads * (p.small ? 16 / (long long)element_size(type) : 16);
-  const int tiles = (int)((num_values + tile - 1) / tile);
-  const long long wanted = std::min<long long>({std::max<long long>(1, kResident / rows), 256, std::max<long long>(1, kMostCandidates / ((long long)num_beams * most))});
-  p.each = (int)((tiles + wanted - 1) / wanted);
+  const int tiles = (num_values + kThreads * kEach - 1) / (kThreads * kEach), most = std::min(num, num_values);
+  const int wanted = (int)std::max<long long>(1, std::min<long long>({kResident / rows, kMostParts, kMostCandidates / ((long long)num_beams * most)}));
+  SelectPlan p;
+  p.each = (tiles + wanted - 1) / wanted;
   p.parts = (tiles + p.each - 1) / p.each;
   return p;
 }
@@ -564,7 +577,7 @@ extern "C" {
 
 long long cuhnsw_select_beams_workspace(int type, int num_batch, int num_beams, int num_values, int num) {
   if (!known_type(type) || num_batch <= 0 || num_beams <= 0 || num_values <= 0 || num <= 0) return 0;
-  return (long long)SelectScratch(nullptr, (long long)num_batch * num_beams, select_plan(type, num_batch, num_beams, num_values, num).parts,
+  return (long long)SelectScratch(nullptr, (long long)num_batch * num_beams, select_plan(num_batch, num_beams, num_values, num).parts,
                                   std::min(num, num_values)).bytes;
 }
 
@@ -582,7 +595,7 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
     if (num_batch == 0) return;
     want(scores && out_totals && out_parents && out_tokens, "select: null argument");
     want(!finished || (end >= 0 && end < num_values), "select: the token that ends a sequence is outside the vocabulary");
-    const SelectPlan p = select_plan(type, num_batch, num_beams, num_values, num);
+    const SelectPlan p = select_plan(num_batch, num_beams, num_values, num);
     const long long rows = (long long)num_batch * num_beams;
     const SelectScratch w(workspace, rows, p.parts, std::min(num, num_values));
     want(workspace && workspace_bytes >= (long long)w.bytes, "select: the workspace is too small");
@@ -593,10 +606,8 @@ int cuhnsw_select_beams(const void* scores, int type, long long stride_b, long l
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const dim3 grid((unsigned)(rows * p.parts));
-      if (p.small && normalise) hipLaunchKernelGGL((select_part_kernel<T, 1, true>), grid, dim3(kThreads), 0, s, a);
-      else if (p.small) hipLaunchKernelGGL((select_part_kernel<T, 1, false>), grid, dim3(kThreads), 0, s, a);
-      else if (normalise) hipLaunchKernelGGL((select_part_kernel<T, sizeof(T), true>), grid, dim3(kThreads), 0, s, a);
-      else hipLaunchKernelGGL((select_part_kernel<T, sizeof(T), false>), grid, dim3(kThreads), 0, s, a);
+      if (normalise) hipLaunchKernelGGL((select_part_kernel<T, true>), grid, dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((select_part_kernel<T, false>), grid, dim3(kThreads), 0, s, a);
     });
     const int candidates = num_beams * p.parts * a.most;
     if (candidates <= 2 * kMerge) hipLaunchKernelGGL(select_merge_kernel<2>, dim3((unsigned)num_batch), dim3(kMerge), (size_t)num_beams * 16, s, a);
