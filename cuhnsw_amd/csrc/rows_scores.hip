@@ -645,7 +645,17 @@ __global__ void __launch_bounds__(64 * kManyWaves, 3) scores_many_kernel(ScoresA
 inline int units_of(int num_dims) { return (num_dims + kUnit - 1) / kUnit; }
 inline int planes_of(int query_type) { return query_type == TYPE_F32 ? 2 : 1; }
 
-// How a call is spread.
+// How a call is spread.  Times in us, both sides of each rule:
+//
+// Many queries' kernel from 384 pairs of a workgroup's rows (128) and a query tile (16) on, where it fills the machine.  16 384 x 1024
+// bf16: 17 queries (256 pairs) 10.4 few, 11.9 many; 33 (384): 13.3, 13.2; 64: 15.2, 13.6; 256: 32.0, 19.0.  16 384 x 960 fp32, 33
+// queries: 18.3, 16.4.  32 000 x 128 fp16, 17 queries (500): 6.4, 5.9.
+//
+// One or two queries are laid out by every workgroup, more by a launch of their own.  100 000 x 50 fp32: 1 query 4.7 and 6.4, 4 queries
+// 8.4 and 7.2; 131 072 x 1024 bf16: 19.8 and 22.7, 25.9 and 22.7.
+//
+// Wavefronts that share a row's elements: doubled while the rows make fewer than 4096 of them (four on a SIMD).  One bf16 query, 16 384 x
+// 4096: one 28.7, eight 11.9; 65 536 x 4096: one 37.2, four 32.4, eight 43.0; 262 144 x 1024: one 30.6, eight 73.1.
 struct ScoresPlan {
   int chunk, padded_units, planes, groups;  // units of a chunk; of a row, with the units that fill the last chunk up
   int query_tiles;                          // of a workgroup; 0: few queries
@@ -659,7 +669,7 @@ struct ScoresPlan {
     groups = (num_dims + group - 1) / group;
     query_blocks = (tiles + 3) / 4;
     const long long blocks = (num_rows + kManyWaves * 32 - 1) / (kManyWaves * 32);
-    query_tiles = tiles > 1 && blocks * query_blocks >= 256 ? (tiles + query_blocks - 1) / query_blocks : 0;
+    query_tiles = tiles > 1 && blocks * tiles >= 384 ? (tiles + query_blocks - 1) / query_blocks : 0;
     own = false;
     lds = 0;
     blocks_each = 1;
@@ -690,7 +700,7 @@ struct ScoresPlan {
     padded_units = (units + chunk - 1) / chunk * chunk;
     if (!query_tiles) {
       const size_t laid_out = (size_t)padded_units * kUnit * std::min(num_queries, kTile) * planes * 2 + (size_t)groups * kTile * 4 + kTile + 32;
-      own = tiles == 1 && laid_out <= 32768;
+      own = num_queries <= 2 && laid_out <= 32768;
       lds = (own ? (laid_out + 15) / 16 * 16 : 0) + (size_t)(split > 1 ? (split - 1) * (waves / split) : 0) * kRowTiles * 64 * sizeof(float4_t);
     }
   }
