@@ -214,3 +214,47 @@ def test_scores_in_a_graph_and_on_another_stream():
       out = packed.scores(late)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, packed.scores(q * 3))
+
+
+def test_more_rows_than_one_launch_packs():
+  from cuhnsw_amd import rows
+  n = (1 << 29) + 5
+  x = torch.empty(n, 1, dtype=torch.float16, device="cuda").fill_(3.5)
+  x[-5:, 0] = torch.tensor([0.0, -7.0, 1.0, 14.0, -0.5], device="cuda")
+  packed, last = rows.pack(x), rows.pack(x[-5:])
+  assert torch.equal(packed.codes[-5:], last.codes) and torch.equal(packed.scales[-5:], last.scales)
+  assert (packed.scales[:-5] == 0.5).all() and (packed.codes[:-5, 0] == 15).all() and not packed.codes[:-5, 1:].any()
+
+
+def test_search_of_no_rows():
+  from cuhnsw_amd import rows
+  packed = rows.pack(torch.zeros(0, 40, device="cuda"))
+  for dist_type in ("dot", "l2"):
+    ids, dist, found = packed.search_knn(torch.ones(3, 40, device="cuda"), 4, dist_type)
+    assert (ids == -1).all() and (dist == float("inf")).all() and (found == 0).all() and ids.shape == dist.shape == (3, 4)
+
+
+def test_search_by_length_in_a_graph_first_and_on_another_stream_then():
+  """The rows' lengths are made when they are first wanted: not to be kept from a capture, and there for every stream."""
+  from cuhnsw_amd import rows
+  g = torch.Generator().manual_seed(2)
+  packed, q = rows.pack(torch.randn(5000, 96, generator=g).cuda()), torch.randn(6, 96, generator=g).cuda()
+  want = rows.PackedRows(packed.codes, packed.scales, num_dims=96).search_knn(q, 5, "l2")
+  packed.scores(q)
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    out = packed.search_knn(q, 5, "l2")
+  other = torch.cuda.Stream()
+  other.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(other):
+    eager = packed.search_knn(q, 5, "l2")
+  here = packed.search_knn(q, 5, "l2")
+  torch.cuda.synchronize()
+  for _ in range(3):
+    for x in out:
+      x.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b, c, d in zip(out, want, eager, here):
+      assert torch.equal(a, b) and torch.equal(c, b) and torch.equal(d, b)

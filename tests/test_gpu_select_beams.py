@@ -233,3 +233,27 @@ def test_selection_and_reordering_in_a_graph():
     for _, out in graphs:
       for a, b in zip(out, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("b, k, v, num", [(1, 16, 5000, 256), (2, 4, 70_000, 256), (1, 1, 400_000, 256), (3, 64, 3000, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_lists_full_of_good_candidates(b, k, v, num, dtype):
+  """All lists are as good as each other, so that most of what is in them reaches a first guess of the bar."""
+  _check(_scores(b, k, v, dtype), None, num, normalise=False)
+
+
+def test_more_equal_totals_than_are_held():
+  x = torch.zeros(2, 64, 1000).cuda()      # 4096 candidates of each batch entry, all with the same total
+  _check(x, None, 64, normalise=False)
+  x[1, 40, 7] = 1.0
+  x[1, 50:, ::3] = -1.0
+  _check(x, torch.zeros(2, 64).cuda(), 64, normalise=False)
+
+
+def test_more_batch_entries_than_a_launch_holds():
+  from cuhnsw_amd import rows
+  b = (1 << 22) + 4321
+  x = torch.randint(-4, 4, (b, 1, 3), generator=torch.Generator().manual_seed(8)).float().cuda()
+  totals, parents, tokens = rows.select_beams(x, None, 2, normalise=False)
+  want = torch.sort(x[:, 0], dim=1, descending=True, stable=True)
+  assert torch.equal(totals, want.values[:, :2]) and torch.equal(tokens.long(), want.indices[:, :2]) and not parents.any()
