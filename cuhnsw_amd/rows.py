@@ -8,7 +8,8 @@
   reorder_states(states, parents)  the beams' states in their new order
 
 Every call runs on its tensors' device and torch's current stream there, does not wait for the GPU, takes its scratch
-memory from torch, and may be captured into a graph.  Wrong arguments are a ValueError (a TypeError where the kind of
+memory from torch, and may be captured into a graph (pack_index waits, and may not; PackedRows.norms waits once).  lookup
+is differentiable, the others are not: their results carry no gradient.  Wrong arguments are a ValueError (a TypeError where the kind of
 object is wrong); what the native library refuses is a RuntimeError with its message, as everywhere in this package.
 There is no CPU form.
 
@@ -248,14 +249,19 @@ class PackedRows:
     return (values - 8.0) * scales if self.offsets is None else values * scales + self.offsets.float()[:, column]
 
   def norms(self):
-    """Squared lengths of the rows, float32 (computed once: the rows must not change afterwards)."""
+    """Squared lengths of the rows, float32.  Computed and waited for once, for every stream (the rows must not change
+    afterwards); inside a capture they belong to the graph and are not kept."""
     if self._norms is None:
-      out = torch.empty(self.num_rows, dtype=torch.float32, device=self.codes.device)
+      device = self.codes.device
+      out = torch.empty(self.num_rows, dtype=torch.float32, device=device)
       step = max(1, (64 << 20) // self.num_dims)
       for low in range(0, self.num_rows, step):
         part = PackedRows(self.codes[low:low + step], self.scales[low:low + step],
                           None if self.offsets is None else self.offsets[low:low + step], num_dims=self.num_dims, group=self.group)
         out[low:low + step] = part.unpack().double().square_().sum(1)
+      if torch.cuda.is_current_stream_capturing():
+        return out
+      torch.cuda.current_stream(device).synchronize()
       self._norms = out
     return self._norms
 
@@ -268,6 +274,9 @@ class PackedRows:
     _check(q.dim() == 2 and q.shape[1] == self.num_dims, "queries have the shape [num_queries, %d]", self.num_dims)
     _check(isinstance(topk, int) and 0 < topk <= 256, "topk is between 1 and 256")
     _same_device(self.codes, q)
+    if self.num_rows == 0:
+      return (q.new_full((q.shape[0], topk), -1, dtype=torch.int32 if self.labels is None else torch.int64),
+              q.new_full((q.shape[0], topk), float("inf"), dtype=torch.float32), q.new_zeros(q.shape[0], dtype=torch.int32))
     l2 = dist_type == "l2"
     bias = -self.norms() if l2 else None
     lengths = q.double().square().sum(1, keepdim=True) if l2 else None
