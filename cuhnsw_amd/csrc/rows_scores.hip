@@ -304,59 +304,72 @@ template <int RT, int MT>
 __device__ inline void store_scores(const ScoresArgs& a, const float4_t (&acc)[RT][MT], int tile0, int c, long long row, const uint32_t (&exponents)[MT],
                                     const float (&bias)[RT]) {
   const int l = threadIdx.x & 3;
-  const long long first = row - l * RT;  // of the four lanes' rows
+  float y[MT][4][RT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    auto score = [&](int r, int t) { return fmaf(a.alpha, ldexpf(acc[t][m][r], (signed char)(exponents[m] >> (8 * r))), bias[t]); };
-    if (a.out_type == TYPE_F32) {
-      const int rows = (int)max(0ll, min((long long)RT, a.num_rows - row));
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int exponent = (signed char)(exponents[m] >> (8 * r));
+#pragma unroll
+      for (int t = 0; t < RT; ++t) y[m][r][t] = fmaf(a.alpha, ldexpf(acc[t][m][r], exponent), bias[t]);
+    }
+  if (a.out_type == TYPE_F32) {
+    const int rows = (int)max(0ll, min((long long)RT, a.num_rows - row));
+    float* to = static_cast<float*>(a.out) + (tile0 * kTile + c * 4) * a.out_stride + row;
+#pragma unroll
+    for (int m = 0; m < MT; ++m, to += kTile * a.out_stride)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int query = (tile0 + m) * kTile + c * 4 + r;
-        LoosePack<float, RT> y;
+        LoosePack<float, RT> together;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) y.at[t] = score(r, t);
-        float* to = static_cast<float*>(a.out) + query * a.out_stride + row;
-        if (query < a.num_queries) {
+        for (int t = 0; t < RT; ++t) together.at[t] = y[m][r][t];
+        if ((tile0 + m) * kTile + c * 4 + r < a.num_queries) {
           if (rows == RT) {
-            *reinterpret_cast<LoosePack<float, RT>*>(to) = y;
+            *reinterpret_cast<LoosePack<float, RT>*>(to + r * a.out_stride) = together;
           } else {
 #pragma unroll
             for (int t = 0; t < RT; ++t)
-              if (t < rows) to[t] = y.at[t];
+              if (t < rows) to[r * a.out_stride + t] = together.at[t];
           }
         }
       }
+    return;
+  }
+  uint32_t words[MT][RT / 2][4];  // two rows in a word
+  auto round_all = [&](auto* two) {
+    using Two = std::remove_pointer_t<decltype(two)>;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int w = 0; w < RT / 2; ++w)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          words[m][w][r] = __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{y[m][r][2 * w], y[m][r][2 * w + 1]}), Two));
+  };
+  if (a.out_type == TYPE_BF16) round_all(static_cast<bfloat2_t*>(nullptr));
+  else round_all(static_cast<half2_t*>(nullptr));
+  const long long first = row - l * RT;  // of the four lanes' rows
+  const int rows = (int)max(0ll, min(4ll * RT, a.num_rows - first));
+  uint16_t* to = static_cast<uint16_t*>(a.out) + (tile0 * kTile + c * 4 + l) * a.out_stride + first;
+#pragma unroll
+  for (int m = 0; m < MT; ++m, to += kTile * a.out_stride) {
+#pragma unroll
+    for (int w = 0; w < RT / 2; ++w) transpose_quad(words[m][w]);
+    if ((tile0 + m) * kTile + c * 4 + l >= a.num_queries) continue;
+    if (rows == 4 * RT) {
+#pragma unroll
+      for (int i = 0; i < RT / 2; ++i) {
+        struct __attribute__((packed, aligned(2))) Loose128 {
+          uint32_t at[4];
+        } eight;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) eight.at[e] = words[m][(i * 4 + e) % (RT / 2)][(i * 4 + e) / (RT / 2)];
+        *reinterpret_cast<Loose128*>(to + i * 8) = eight;
+      }
     } else {
-      const int query = (tile0 + m) * kTile + c * 4 + l, rows = (int)max(0ll, min(4ll * RT, a.num_rows - first));
-      const bool there = query < a.num_queries && rows > 0;
-      uint32_t words[RT / 2][4];  // two rows in a word
 #pragma unroll
-      for (int w = 0; w < RT / 2; ++w) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float low = score(r, 2 * w), high = score(r, 2 * w + 1);
-          words[w][r] = a.out_type == TYPE_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{low, high}), bfloat2_t))
-                                                : __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{low, high}), half2_t));
-        }
-        transpose_quad(words[w]);
-      }
-      uint16_t* to = static_cast<uint16_t*>(a.out) + query * a.out_stride + first;
-      if (there && rows == 4 * RT) {
-#pragma unroll
-        for (int i = 0; i < RT / 2; ++i) {
-          struct __attribute__((packed, aligned(2))) Loose128 {
-            uint32_t at[4];
-          } eight;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) eight.at[e] = words[(i * 4 + e) % (RT / 2)][(i * 4 + e) / (RT / 2)];
-          *reinterpret_cast<Loose128*>(to + i * 8) = eight;
-        }
-      } else if (there) {
-#pragma unroll
-        for (int i = 0; i < 4 * RT; ++i)
-          if (i < rows) to[i] = (uint16_t)(words[i / 2 % (RT / 2)][i / 2 / (RT / 2)] >> (i % 2 * 16));
-      }
+      for (int i = 0; i < 4 * RT; ++i)
+        if (i < rows) to[i] = (uint16_t)(words[m][i / 2 % (RT / 2)][i / 2 / (RT / 2)] >> (i % 2 * 16));
     }
   }
 }
