@@ -146,7 +146,8 @@ def lookup(table, ids, scale=1.0, dtype=None):
 
   table: [rows, dims], float32, float16 or bfloat16, rows contiguous; ids: int32 or int64 of any shape; the result, of
   shape [*ids.shape, dims], has the table's type or is float32.  Products are taken in 32 bits and rounded once.
-  Differentiable with respect to table (once): see lookup_grad."""
+  Differentiable with respect to table (once): see lookup_grad.  Where a backward pass is captured into a graph, no eager
+  graph over the same table may be alive (its leaf belongs to another stream then, which torch would wait for)."""
   _tensor(table, "table", 2)
   _tensor(ids, "ids", types=_IDS)
   scale = _number(scale, "scale")
