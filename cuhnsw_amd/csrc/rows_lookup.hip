@@ -123,7 +123,9 @@ void launch_lookup(const LookupArgs& a, hipStream_t stream) {
 // A stable sort of (id, place) by id, least significant digit first: places of one id stay in ascending order, so the sums do
 // not depend on how the work was spread.  Ids outside the table take the key num_rows, behind all others.  One pass is two
 // launches: every workgroup counts the digits of its stretch of ids; then each adds up the counts of the others before it,
-// and each of its wavefronts ranks a quarter of the stretch by ballots among the lanes that hold the same digit.
+// and each of its wavefronts ranks a quarter of the stretch by ballots among the lanes that hold the same digit.  65 536 ids of
+// 17 bits: twice 4.8 + 12.2 us, all of it waits; with stretches of 512 or 2048 ids instead of 1024 the second launch takes
+// 13.8 and 14.3.
 constexpr int kSortThreads = 256, kSortWaves = 4, kSortBlocks = 128, kMostDigits = 2048;
 
 struct SortPlan {
