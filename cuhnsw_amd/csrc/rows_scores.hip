@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(512) scores_few_kernel(ScoresArgs a) {
 // together.
 //
 // What bounds it: instructions of the vector units.  For every matrix product of 16 x 16 x 32 a quarter of a word comes apart
-// and four sums are scaled (four more with offsets).  131 072 x 1024 by 1024 bfloat16 queries: 366 us, 752 TFLOP/s (a library's product
+// and four sums are scaled (four more with offsets).  131 072 x 1024 by 1024 bfloat16 queries: 371 us, 741 TFLOP/s (a library's product
 // in float16 reaches 1128 here); 200 003 x 960 by 33 float32 queries with offsets (two planes): 74 us, of which vector instructions 38 and
 // matrix products 16; 500 000 x 128 by 256 with offsets: 107 us, 68 of them without
 // the stores of its 256 MB of scores, which the next block's work hides little of: a wavefront waits for them before it uses what was
