@@ -575,7 +575,8 @@ __global__ void __launch_bounds__(64 * kManyWaves, 3) scores_many_kernel(ScoresA
     }
     if (!CENTRED && wave < MT) {  // the sums of the chunk's groups, a float for each lane
       const size_t tile = min(query_block * MT + wave, last_tile);
-      const int at = min(chunk * UC / GU * kTile + lane, a.groups * kTile - 1);  // (what is not the chunk's is not looked at)
+      // (behind the row's last group the query's own sum of that one: it meets an offset of 0, and 0 times what is not finite is not 0)
+      const int at = min(chunk * UC / GU + lane / kTile, a.groups - 1) * kTile + lane % kTile;
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(a.sums + tile * a.groups * kTile + at)),
                                        (__attribute__((address_space(3))) void*)&sums[buffer][wave][0], 4, 0, 0);
     }
