@@ -23,7 +23,7 @@ SYMBOLS = [
     "cuhnsw_get_items", "cuhnsw_search_items", "cuhnsw_get_labels", "cuhnsw_pack_items", "cuhnsw_lookup_rows",
     "cuhnsw_lookup_grad_workspace", "cuhnsw_lookup_rows_grad", "cuhnsw_pack_rows", "cuhnsw_packed_scores_workspace",
     "cuhnsw_packed_scores", "cuhnsw_select_beams_workspace", "cuhnsw_select_beams", "cuhnsw_reorder_states",
-    "cuhnsw_use_device",
+    "cuhnsw_use_device", "cuhnsw_packed_scores_plan",
 ]
 
 _lib = None
@@ -84,6 +84,7 @@ def load():
   l.cuhnsw_pack_rows.argtypes = [vp, ci, ll, ll, ci, ci, vp, vp, vp, ci, vp]
   l.cuhnsw_packed_scores_workspace.argtypes = [ll, ci, ci, ci, ci]
   l.cuhnsw_packed_scores_workspace.restype = ll
+  l.cuhnsw_packed_scores_plan.argtypes = [ll, ci, ci, ci, ci, vp]
   l.cuhnsw_packed_scores.argtypes = [vp, vp, vp, ci, ll, ci, ci, vp, ci, ll, ci, cf, vp, vp, ci, ll, vp, ll, vp]
   l.cuhnsw_select_beams_workspace.argtypes = [ci, ci, ci, ci, ci]
   l.cuhnsw_select_beams_workspace.restype = ll

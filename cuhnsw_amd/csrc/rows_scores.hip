@@ -819,6 +819,16 @@ long long cuhnsw_packed_scores_workspace(long long num_rows, int num_dims, int g
   return (long long)ScoresScratch(nullptr, num_queries, ScoresPlan(num_rows, num_dims, group, query_type, num_queries)).bytes;
 }
 
+int cuhnsw_packed_scores_plan(long long num_rows, int num_dims, int group, int query_type, int num_queries, int* out) {
+  if (num_rows <= 0 || num_dims <= 0 || group <= 0 || !known_type(query_type) || num_queries <= 0 || !out) return -1;
+  const ScoresPlan p(num_rows, num_dims, group, query_type, num_queries);
+  out[0] = p.query_tiles;
+  out[1] = p.blocks_each;
+  out[2] = p.split;
+  out[3] = p.own;
+  return 0;
+}
+
 int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offsets, int scale_type, long long num_rows, int num_dims,
                          int group, const void* queries, int query_type, long long query_stride, int num_queries, float alpha,
                          const float* bias, void* out, int out_type, long long out_stride, void* workspace, long long workspace_bytes,

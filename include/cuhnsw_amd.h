@@ -314,10 +314,15 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
  *
  * cuhnsw_pack_rows: the nearest such rows of finite ones (scale = largest magnitude / 7, or the span / 15 with offsets).
  * cuhnsw_packed_scores: out[m][n] = alpha * <row n, query m> + bias[n] (bias: float32 [num_rows] or NULL), of the queries'
- *   type or float32.  A query that holds an infinity or a NaN gets NaN or infinities; other queries are not touched by it. */
+ *   type or float32.  A query that holds an infinity or a NaN gets NaN or infinities; other queries are not touched by it.
+ * cuhnsw_packed_scores_plan: how such a call goes, in four numbers: [0] tiles of 16 queries that a wavefront of the kernel for
+ *   many queries has at a time, 0 where the call goes to the kernel for few; [1] blocks of these tiles that its workgroup goes
+ *   over; [2] wavefronts of the kernel for few that share a row; [3] whether its workgroups lay the queries out themselves.
+ *   -1 for bad sizes. */
 int cuhnsw_pack_rows(const void* rows, int type, long long row_stride, long long num_rows, int num_dims, int group, void* codes,
                      void* scales, void* offsets, int scale_type, void* stream);
 long long cuhnsw_packed_scores_workspace(long long num_rows, int num_dims, int group, int query_type, int num_queries);
+int cuhnsw_packed_scores_plan(long long num_rows, int num_dims, int group, int query_type, int num_queries, int* out);
 int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offsets, int scale_type, long long num_rows, int num_dims,
                          int group, const void* queries, int query_type, long long query_stride, int num_queries, float alpha,
                          const float* bias, void* out, int out_type, long long out_stride, void* workspace, long long workspace_bytes,
