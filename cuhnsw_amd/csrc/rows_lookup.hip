@@ -312,15 +312,27 @@ struct GradArgs {
   float scale;
   void* out;
   int lanes, rows;  // lanes that share a row, rows of a workgroup
+  int first_block;  // of this launch
 };
+// A launch has fewer than 2^32 threads: what more workgroups have to do goes in several.
+constexpr long long kMostBlocks = 0xffffff;
+template <typename F>
+void in_launches(GradArgs& g, long long blocks, F&& launch) {
+  for (long long first = 0; first < blocks; first += kMostBlocks) {
+    g.first_block = (int)first;
+    launch(dim3((unsigned)std::min(kMostBlocks, blocks - first)));
+    HIP_CHECK(hipGetLastError());  // (what comes next reads what this one writes)
+  }
+}
 
 // Stretches of the sorted list that are one id's alone; and, by the workgroups behind those, where the rows of grad_kernel's
 // workgroups begin: a search for each thread, which would be every one's first wait there.
 template <typename T, int VE>
 __global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
   __shared__ float parts[256 * VE];
-  if ((int)blockIdx.x >= a.num_stretches) {
-    const int i = (blockIdx.x - a.num_stretches) * 256 + threadIdx.x;
+  const int block = a.first_block + blockIdx.x;
+  if (block >= a.num_stretches) {
+    const int i = (block - a.num_stretches) * 256 + threadIdx.x;
     if (i > a.num_blocks) return;
     const int row = (int)min((long long)i * a.rows, (long long)a.num_rows);
     int low = 0, high = a.num_ids;
@@ -332,7 +344,7 @@ __global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
     a.bounds[i] = low;
     return;
   }
-  const int first = blockIdx.x * kLong, key = a.keys[first];
+  const int first = block * kLong, key = a.keys[first];
   if (key >= a.num_rows || a.keys[first + kLong - 1] != key) return;
   const int lane = threadIdx.x & (a.lanes - 1), vectors = vectors_of<VE>(a.num_dims);
   const T* grad = static_cast<const T*>(a.grad);
@@ -342,7 +354,7 @@ __global__ void __launch_bounds__(256) grad_long_kernel(GradArgs a) {
     sum_items_together<T, VE>(kLong, a.lanes, [&](int i) {
       return reinterpret_cast<const LoosePack<T, VE>*>(grad + (long long)a.places[first + i] * a.grad_stride + d);
     }, sum, parts);
-    if (threadIdx.x < a.lanes) store<false>(a.long_sums + (long long)blockIdx.x * a.num_dims + d, sum, 1.f);
+    if (threadIdx.x < a.lanes) store<false>(a.long_sums + (long long)block * a.num_dims + d, sum, 1.f);
   }
 }
 
@@ -354,7 +366,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
   __shared__ float parts[256 * VE];
   extern __shared__ uint64_t picked[];  // few ids: [num_ids], and their places in order behind them
   int* in_order = reinterpret_cast<int*>(picked + (FEW ? a.num_ids : 0));
-  const int tid = threadIdx.x, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.num_rows - row0);
+  const int tid = threadIdx.x, block = a.first_block + blockIdx.x, row0 = block * a.rows, rows = min(a.rows, a.num_rows - row0);
   for (int r = tid; r < rows; r += 256) first[r] = last[r] = 0;
   if (tid == 0) long_count = 0;
   if (FEW) {
@@ -403,7 +415,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs a) {
     __syncthreads();
     for (int i = tid; i < count; i += 256) in_order[i] = (int)(uint32_t)picked[in_order[i]];
   } else {
-    const int begin = a.bounds[blockIdx.x], end = a.bounds[blockIdx.x + 1];
+    const int begin = a.bounds[block], end = a.bounds[block + 1];
     __syncthreads();
     for (int i = begin + tid; i < end; i += 256) {
       const int key = a.keys[i];
@@ -526,10 +538,17 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
     g.scale = scale;
     g.out = out;
     const bool few = num_ids <= kFew;
+    const SortPlan p = sort_plan(num_ids, num_rows);
+    const GradScratch w(few ? nullptr : workspace, num_ids, num_rows, num_dims, p);
     if (!few) {
-      const SortPlan p = sort_plan(num_ids, num_rows);
-      const GradScratch w(workspace, num_ids, num_rows, num_dims, p);
       want(workspace && workspace_bytes >= (long long)w.bytes, "lookup gradient: the workspace is too small");
+      g.keys = w.keys[(p.passes - 1) & 1];
+      g.places = w.places[(p.passes - 1) & 1];
+      g.long_sums = w.long_sums;
+      g.bounds = w.bounds;
+      g.num_stretches = (int)(num_ids / kLong);
+    }
+    auto sort_ids = [&] {
       for (int pass = 0; pass < p.passes; ++pass) {
         const SortInput in{ids, ids_64, (int)num_rows, pass ? w.keys[(pass - 1) & 1] : nullptr, pass ? w.places[(pass - 1) & 1] : nullptr};
         hipLaunchKernelGGL(sort_count_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, in, (int)num_ids, p.chunk, pass * p.bits, 1 << p.bits,
@@ -537,12 +556,8 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
         hipLaunchKernelGGL(sort_place_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, in, (int)num_ids, p.chunk, pass * p.bits, 1 << p.bits,
                            p.bits, w.counts, w.keys[pass & 1], w.places[pass & 1]);
       }
-      g.keys = w.keys[(p.passes - 1) & 1];
-      g.places = w.places[(p.passes - 1) & 1];
-      g.long_sums = w.long_sums;
-      g.bounds = w.bounds;
-      g.num_stretches = (int)(num_ids / kLong);
-    }
+      HIP_CHECK(hipGetLastError());
+    };
     with_type(grad_type, [&](auto* t) {
       with_type(out_type, [&](auto* u) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -556,14 +571,17 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
             const long long bytes = (long long)num_dims * (sizeof(U) + sizeof(T) * (num_ids / num_rows));
             g.rows = (int)std::min<long long>(kMostRows, std::max<long long>(groups, 32768 / bytes / groups * groups));
             g.num_blocks = (int)((num_rows + g.rows - 1) / g.rows);
-            want(g.num_blocks <= 0xffffff, "lookup gradient: too many rows");  // (a launch has fewer than 2^32 threads)
-            const dim3 grid((unsigned)g.num_blocks);
-            if (!few)
-              hipLaunchKernelGGL((grad_long_kernel<T, VE>), dim3((unsigned)(g.num_stretches + g.num_blocks / 256 + 1)), dim3(256), 0, s, g);
+            if (!few) {
+              sort_ids();
+              in_launches(g, (long long)g.num_stretches + g.num_blocks / 256 + 1,
+                          [&](dim3 grid) { hipLaunchKernelGGL((grad_long_kernel<T, VE>), grid, dim3(256), 0, s, g); });
+            }
             with_flag(num_rows * num_dims * (long long)sizeof(U) >= kStreamedFrom, [&](auto streamed) {
               constexpr bool kStreamed = decltype(streamed)::value;
-              if (few) hipLaunchKernelGGL((grad_kernel<T, U, VE, true, kStreamed>), grid, dim3(256), (size_t)num_ids * 12, s, g);
-              else hipLaunchKernelGGL((grad_kernel<T, U, VE, false, kStreamed>), grid, dim3(256), 0, s, g);
+              in_launches(g, g.num_blocks, [&](dim3 grid) {
+                if (few) hipLaunchKernelGGL((grad_kernel<T, U, VE, true, kStreamed>), grid, dim3(256), (size_t)num_ids * 12, s, g);
+                else hipLaunchKernelGGL((grad_kernel<T, U, VE, false, kStreamed>), grid, dim3(256), 0, s, g);
+              });
             });
           });
         } else {
@@ -571,7 +589,6 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
         }
       });
     });
-    HIP_CHECK(hipGetLastError());
   });
 }
 
