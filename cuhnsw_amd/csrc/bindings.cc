@@ -91,14 +91,14 @@ class CuHNSWBind {
     int_array _items(items);
     float_array _out(out);
     if (_items.ndim() != 1) throw std::runtime_error("items must be 1d array");
-    if ((long long)_out.size() < (long long)_items.size() * cuhnsw_num_dims(obj_)) throw std::runtime_error("output array is too small");
+    if (_out.ndim() != 2 || _out.shape(0) != _items.size()) throw std::runtime_error("output must be a 2d array with a row for every item");
     const int* in = _items.data();
     float* to = _out.mutable_data();
-    const int num = (int)_items.size();
+    const int num = (int)_items.size(), dims = (int)_out.shape(1);
     int rc;
     {
       py::gil_scoped_release release;
-      rc = cuhnsw_get_items(obj_, in, num, scale, to);
+      rc = cuhnsw_get_items(obj_, in, num, dims, scale, to);
     }
     Check(rc);
   }
@@ -123,8 +123,9 @@ class CuHNSWBind {
     Check(rc);
   }
   py::array_t<long long> GetLabels() {
-    py::array_t<long long> out(cuhnsw_num_data(obj_));
-    Check(cuhnsw_get_labels(obj_, out.mutable_data()));
+    const int num = cuhnsw_num_data(obj_);
+    py::array_t<long long> out(num);
+    Check(cuhnsw_get_labels(obj_, num, out.mutable_data()));
     return out;
   }
   void PackItems(int group, uintptr_t codes, uintptr_t scales, uintptr_t offsets, int scale_type, uintptr_t stream) {

@@ -154,15 +154,15 @@ int cuhnsw_search_knn_device_noalloc(cuhnsw_engine* e, const float* d_qdata, int
     g.search_device(d_qdata, num_queries, topk, ef_search, d_nns, d_distances, d_found_cnt, nullptr, kernel_ms, true);
   });
 }
-int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, float scale, float* out) {
-  return guarded(e, [&](Engine& g) { e->items.get(g, items, num_items, scale, out); });
+int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, int num_dims, float scale, float* out) {
+  return guarded(e, [&](Engine& g) { e->items.get(g, items, num_items, num_dims, scale, out); });
 }
 int cuhnsw_search_items(cuhnsw_engine* e, const int* items, int num_items, float scale, int topk, int ef_search, int* nns,
                         float* distances, int* found_cnt) {
   return guarded(e, [&](Engine& g) { e->items.search(g, items, num_items, scale, topk, ef_search, nns, distances, found_cnt); });
 }
-int cuhnsw_get_labels(cuhnsw_engine* e, long long* out) {
-  return guarded(e, [&](Engine& g) { e->items.labels(g, out); });
+int cuhnsw_get_labels(cuhnsw_engine* e, int num_rows, long long* out) {
+  return guarded(e, [&](Engine& g) { e->items.labels(g, num_rows, out); });
 }
 int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, void* offsets, int scale_type, void* stream) {
   return guarded(e, [&](Engine& g) { e->items.pack(g, group, codes, scales, offsets, scale_type, static_cast<hipStream_t>(stream)); });

@@ -13,7 +13,8 @@ class Items {
   // the index was replaced
   void forget() { label_order_.clear(); }
 
-  void labels(Engine& g, long long* out) {
+  void labels(Engine& g, int num_rows, long long* out) {
+    same_index(g.host.N, num_rows, "rows");
     need_vectors(g, "get_labels");
     want(out, "get_labels: null argument");
     if (!g.host.labelled) {
@@ -24,7 +25,8 @@ class Items {
     HIP_CHECK(hipStreamSynchronize(g.stream));
   }
 
-  void get(Engine& g, const int* items, int n, float scale, float* out) {
+  void get(Engine& g, const int* items, int n, int num_dims, float scale, float* out) {
+    same_index(g.host.D, num_dims, "elements a vector");
     need_vectors(g, "get_items");
     if (n <= 0) return;
     want(items && out, "get_items: null argument");
@@ -64,6 +66,11 @@ class Items {
   }
 
  private:
+  // Another thread's call may have put another index in the place of the one that the caller made room for.
+  static void same_index(int has, int expected, const char* what) {
+    if (has != expected)
+      throw std::runtime_error("the index was replaced meanwhile: " + std::to_string(has) + " " + what + ", not " + std::to_string(expected));
+  }
   static void need_vectors(const Engine& g, const char* what) {
     g.need_device();
     if (!g.have_data) throw std::runtime_error(std::string(what) + ": no vectors (call set_data or load_index first)");
@@ -74,7 +81,7 @@ class Items {
     std::vector<int> rows(items, items + n);
     if (g.host.labelled && label_order_.empty()) {
       std::vector<long long> labels_of((size_t)g.host.N);
-      labels(g, labels_of.data());
+      labels(g, g.host.N, labels_of.data());
       std::vector<std::pair<uint64_t, int>> order((size_t)g.host.N);
       for (int i = 0; i < g.host.N; ++i) order[(size_t)i] = {(uint64_t)labels_of[(size_t)i], i};
       std::sort(order.begin(), order.end());

@@ -272,16 +272,19 @@ int cuhnsw_set_tunable(cuhnsw_engine* e, const char* name, double value);
 /* ---- the index's vectors as a table ---------------------------------------------------------------
  * Items are named as a search names them: by label on an index that came from a file, else by row number.
  *
+ * Two threads may share an engine: what a result was made for (num_dims, num_rows) goes with the call, which fails where the
+ * index is another one by now, and writes nothing.
+ *
  * cuhnsw_get_items: out[i][:] = scale * vector of items[i], float32 [num_items, num_dims] (with fp16_storage the
  *   rounded vector).  Host pointers.  An item that is not in the index is an error.
  * cuhnsw_search_items: cuhnsw_search_knn with these vectors as queries; they never leave the GPU.
- * cuhnsw_get_labels: the label of every row (its number where the index did not come from a file).
+ * cuhnsw_get_labels: the label of each of the num_rows rows (its number where the index did not come from a file).
  * cuhnsw_pack_items: all vectors in 4 bits (cuhnsw_pack_rows) into device memory of the caller's, on the caller's
  *   stream (NULL = the default stream); has ended when the call returns. */
-int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, float scale, float* out);
+int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, int num_dims, float scale, float* out);
 int cuhnsw_search_items(cuhnsw_engine* e, const int* items, int num_items, float scale, int topk, int ef_search, int* nns,
                         float* distances, int* found_cnt);
-int cuhnsw_get_labels(cuhnsw_engine* e, long long* out);
+int cuhnsw_get_labels(cuhnsw_engine* e, int num_rows, long long* out);
 int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, void* offsets, int scale_type, void* stream);
 
 /* ---- operators on tables of vectors ----------------------------------------------------------------
