@@ -75,7 +75,7 @@ def load():
   l.cuhnsw_get_items.argtypes = [vp, vp, ci, ci, cf, vp]
   l.cuhnsw_search_items.argtypes = [vp, vp, ci, cf, ci, ci, vp, vp, vp]
   l.cuhnsw_get_labels.argtypes = [vp, ci, vp]
-  l.cuhnsw_pack_items.argtypes = [vp, ci, vp, vp, vp, ci, vp]
+  l.cuhnsw_pack_items.argtypes = [vp, ci, ci, ci, vp, vp, vp, ci, vp, vp, vp]
   l.cuhnsw_use_device.argtypes = [ci, ctypes.POINTER(ci)]
   l.cuhnsw_lookup_rows.argtypes = [vp, ci, ll, ll, ci, vp, ci, ll, cf, vp, ci, vp]
   l.cuhnsw_lookup_grad_workspace.argtypes = [ll, ll, ci]

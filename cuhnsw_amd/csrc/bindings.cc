@@ -128,8 +128,13 @@ class CuHNSWBind {
     Check(cuhnsw_get_labels(obj_, num, out.mutable_data()));
     return out;
   }
-  void PackItems(int group, uintptr_t codes, uintptr_t scales, uintptr_t offsets, int scale_type, uintptr_t stream) {
-    Check(cuhnsw_pack_items(obj_, group, (void*)codes, (void*)scales, (void*)offsets, scale_type, (void*)stream));
+  // the labels and the number of deleted elements of the index that was packed
+  py::tuple PackItems(int num_rows, int num_dims, int group, uintptr_t codes, uintptr_t scales, uintptr_t offsets, int scale_type, uintptr_t stream) {
+    py::array_t<long long> labels(num_rows);
+    int deleted = 0;
+    Check(cuhnsw_pack_items(obj_, num_rows, num_dims, group, (void*)codes, (void*)scales, (void*)offsets, scale_type, labels.mutable_data(), &deleted,
+                            (void*)stream));
+    return py::make_tuple(labels, deleted);
   }
   int NumDeleted() const { return cuhnsw_num_deleted(obj_); }
   void SetTunable(std::string name, double value) {
@@ -255,8 +260,8 @@ PYBIND11_MODULE(cuhnsw_bind, m) {
       .def("search_items", &CuHNSWBind::SearchItems, py::arg("items"), py::arg("scale"), py::arg("topk"), py::arg("ef_search"),
            py::arg("nns"), py::arg("distances"), py::arg("found"))
       .def("get_labels", &CuHNSWBind::GetLabels)
-      .def("pack_items", &CuHNSWBind::PackItems, py::arg("group"), py::arg("codes"), py::arg("scales"), py::arg("offsets"),
-           py::arg("scale_type"), py::arg("stream"))
+      .def("pack_items", &CuHNSWBind::PackItems, py::arg("num_rows"), py::arg("num_dims"), py::arg("group"), py::arg("codes"), py::arg("scales"),
+           py::arg("offsets"), py::arg("scale_type"), py::arg("stream"))
       .def("num_deleted", &CuHNSWBind::NumDeleted)
       .def("num_data", &CuHNSWBind::NumData)
       .def("num_dims", &CuHNSWBind::NumDims)

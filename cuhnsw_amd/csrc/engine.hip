@@ -164,8 +164,13 @@ int cuhnsw_search_items(cuhnsw_engine* e, const int* items, int num_items, float
 int cuhnsw_get_labels(cuhnsw_engine* e, int num_rows, long long* out) {
   return guarded(e, [&](Engine& g) { e->items.labels(g, num_rows, out); });
 }
-int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, void* offsets, int scale_type, void* stream) {
-  return guarded(e, [&](Engine& g) { e->items.pack(g, group, codes, scales, offsets, scale_type, static_cast<hipStream_t>(stream)); });
+int cuhnsw_pack_items(cuhnsw_engine* e, int num_rows, int num_dims, int group, void* codes, void* scales, void* offsets, int scale_type,
+                      long long* labels, int* num_deleted, void* stream) {
+  return guarded(e, [&](Engine& g) {
+    e->items.pack(g, num_rows, num_dims, group, codes, scales, offsets, scale_type, static_cast<hipStream_t>(stream));
+    if (labels) e->items.labels(g, num_rows, labels);
+    if (num_deleted) *num_deleted = g.host.n_deleted;
+  });
 }
 int cuhnsw_debug_gather_probe(cuhnsw_engine* e, int waves_per_cu, int rows_in_flight, int dependent, double* rows,
                               float* ms) {

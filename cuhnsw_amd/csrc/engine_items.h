@@ -52,7 +52,9 @@ class Items {
   }
 
   // On the caller's stream, and waited for: the vectors may be replaced by the next call.
-  void pack(Engine& g, int group, void* codes, void* scales, void* offsets, int scale_type, hipStream_t stream) {
+  void pack(Engine& g, int num_rows, int num_dims, int group, void* codes, void* scales, void* offsets, int scale_type, hipStream_t stream) {
+    same_index(g.host.N, num_rows, "rows");
+    same_index(g.host.D, num_dims, "elements a vector");
     need_vectors(g, "pack_items");
     want(group == 32 || group == 64 || group == 128, "pack_items: the group is 32, 64 or 128 elements");
     want(scale_type == TYPE_F16 || scale_type == TYPE_BF16, "pack_items: scales are float16 or bfloat16");

@@ -324,15 +324,21 @@ def pack_index(index, group=32, offsets=False, scale_dtype=torch.float16):
   """PackedRows of the vectors that a CuHNSW index holds (CuHNSW.pack_rows).  Rows of a loaded index keep its labels; an index
   with deleted elements is refused, since its rows are all returned here."""
   obj = index.obj
-  if obj.num_deleted() > 0:
-    raise RuntimeError("pack_rows: the index holds deleted elements")
-  _check(obj.num_data() > 0, "pack_rows: no vectors (call set_data or load_index first)")
+
+  def refuse_deleted(count):
+    if count > 0:
+      raise RuntimeError("pack_rows: the index holds deleted elements")
+
+  refuse_deleted(obj.num_deleted())
+  n, d = obj.num_data(), obj.num_dims()
+  _check(n > 0, "pack_rows: no vectors (call set_data or load_index first)")
   _check(torch.cuda.is_available(), "no HIP device available: this call needs a GPU")
   device = torch.device("cuda", torch.cuda.current_device())
-  n, d = obj.num_data(), obj.num_dims()
   codes, scales, lows = _empty_packed(n, d, group, offsets, scale_dtype, device)
-  obj.pack_items(group, codes.data_ptr(), scales.data_ptr(), _address(lows), _SCALES[scale_dtype], _raw_stream(device.index))
-  labels = obj.get_labels()
+  # (one call, so that all of it is of one index: another thread may replace it, and where the sizes differ the call fails)
+  labels, deleted = obj.pack_items(n, d, group, codes.data_ptr(), scales.data_ptr(), _address(lows), _SCALES[scale_dtype],
+                                   _raw_stream(device.index))
+  refuse_deleted(deleted)
   plain = np.array_equal(labels, np.arange(n))
   return PackedRows(codes, scales, lows, num_dims=d, group=group, labels=None if plain else torch.from_numpy(labels).to(device))
 

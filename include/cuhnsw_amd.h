@@ -279,13 +279,15 @@ int cuhnsw_set_tunable(cuhnsw_engine* e, const char* name, double value);
  *   rounded vector).  Host pointers.  An item that is not in the index is an error.
  * cuhnsw_search_items: cuhnsw_search_knn with these vectors as queries; they never leave the GPU.
  * cuhnsw_get_labels: the label of each of the num_rows rows (its number where the index did not come from a file).
- * cuhnsw_pack_items: all vectors in 4 bits (cuhnsw_pack_rows) into device memory of the caller's, on the caller's
- *   stream (NULL = the default stream); has ended when the call returns. */
+ * cuhnsw_pack_items: all num_rows vectors of num_dims elements in 4 bits (cuhnsw_pack_rows) into device memory of the
+ *   caller's, on the caller's stream (NULL = the default stream); has ended when the call returns.  Of the same index: the label of
+ *   every row (labels, host memory, or NULL) and how many of the rows are deleted elements (num_deleted, or NULL). */
 int cuhnsw_get_items(cuhnsw_engine* e, const int* items, int num_items, int num_dims, float scale, float* out);
 int cuhnsw_search_items(cuhnsw_engine* e, const int* items, int num_items, float scale, int topk, int ef_search, int* nns,
                         float* distances, int* found_cnt);
 int cuhnsw_get_labels(cuhnsw_engine* e, int num_rows, long long* out);
-int cuhnsw_pack_items(cuhnsw_engine* e, int group, void* codes, void* scales, void* offsets, int scale_type, void* stream);
+int cuhnsw_pack_items(cuhnsw_engine* e, int num_rows, int num_dims, int group, void* codes, void* scales, void* offsets, int scale_type,
+                      long long* labels, int* num_deleted, void* stream);
 
 /* ---- operators on tables of vectors ----------------------------------------------------------------
  * No engine: device pointers of the current HIP device and a hipStream_t (NULL = the default stream).  Unlike the calls
