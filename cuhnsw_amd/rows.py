@@ -21,6 +21,7 @@ import sys
 if "torch" not in sys.modules and "cuhnsw_amd.cuhnsw_bind" in sys.modules:
   raise ImportError("cuhnsw_amd.rows: import torch before cuhnsw_amd (two HIP runtimes would be loaded otherwise)")
 
+import ctypes
 import numbers
 
 import numpy as np
@@ -30,6 +31,20 @@ try:
   from cuhnsw_amd import cuhnsw_bind as _native
 except ImportError as exc:  # pragma: no cover
   raise ImportError("cuhnsw_amd: the native extension is missing (%s); build it with `python -m cuhnsw_amd.build`" % exc) from exc
+
+
+def _one_hip_runtime():
+  """Whether torch and the native library call the same one (not where torch was imported after the library was loaded)."""
+  def runtime_of(module):
+    return ctypes.cast(ctypes.CDLL(module.__file__).hipGetDeviceCount, ctypes.c_void_p).value
+  try:
+    return runtime_of(torch._C) == runtime_of(_native)
+  except AttributeError:  # (a torch without HIP)
+    return True
+
+
+if not _one_hip_runtime():
+  raise ImportError("cuhnsw_amd.rows: import torch before cuhnsw_amd (two HIP runtimes are loaded)")
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _GROUPS = (32, 64, 128)
