@@ -9,7 +9,7 @@
 
 Every call runs on its tensors' device and torch's current stream there, does not wait for the GPU, takes its scratch
 memory from torch, and may be captured into a graph (pack_index waits, and may not; PackedRows.norms waits once).  lookup
-is differentiable, the others are not: their results carry no gradient.  Wrong arguments are a ValueError (a TypeError where the kind of
+is differentiable, the others are not: their results carry no gradient and no tangent.  Wrong arguments are a ValueError (a TypeError where the kind of
 object is wrong); what the native library refuses is a RuntimeError with its message, as everywhere in this package.
 There is no CPU form.
 
@@ -107,12 +107,15 @@ def _flat(ids):
   return ids if ids.is_contiguous() else ids.contiguous()
 
 
-def _lookup(table, flat, scale, dtype, device):
+def _lookup(table, stride, flat, scale, dtype, device):
   dims = table.shape[1]
   out = table.new_empty((flat.shape[0], dims), dtype=dtype)
-  _native.lookup_rows(table.data_ptr(), _TYPES[table.dtype], table.shape[0], _rows(table, "table"), dims, flat.data_ptr(), _IDS[flat.dtype],
+  _native.lookup_rows(table.data_ptr(), _TYPES[table.dtype], table.shape[0], stride, dims, flat.data_ptr(), _IDS[flat.dtype],
                       flat.shape[0], scale, out.data_ptr(), _TYPES[dtype], device, _raw_stream(device))
   return out
+
+
+_tangent = torch.autograd.forward_ad.unpack_dual
 
 
 def _grad_workspace(flat, num_rows, dims):
@@ -137,23 +140,23 @@ class _Lookup(torch.autograd.Function):
   """(What can be found out in the forward pass is: the backward pass runs on autograd's own thread, where Python is slow.)"""
 
   @staticmethod
-  def forward(ctx, table, flat, shape, scale, dtype, device):
+  def forward(ctx, table, stride, flat, shape, scale, dtype, device):
     num_rows, dims = table.shape
     ctx.save_for_backward(flat)
     ctx.rest = num_rows, dims, scale, table.dtype, _grad_workspace(flat, num_rows, dims), device
-    out = _lookup(table, flat, scale, dtype, device)
+    out = _lookup(table, stride, flat, scale, dtype, device)
     return out if shape is None else out.view(shape)
 
   @staticmethod
   def backward(ctx, grad):
     if torch.is_grad_enabled():  # (a graph of the gradient is wanted: one that says that it cannot be had)
       return _Lookup.backward_of_once(ctx, grad)
-    return _lookup_grad(grad, *ctx.saved_tensors, *ctx.rest), None, None, None, None, None
+    return _lookup_grad(grad, *ctx.saved_tensors, *ctx.rest), None, None, None, None, None, None
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward_of_once(ctx, grad):
-    return _lookup_grad(grad, *ctx.saved_tensors, *ctx.rest), None, None, None, None, None
+    return _lookup_grad(grad, *ctx.saved_tensors, *ctx.rest), None, None, None, None, None, None
 
 
 def lookup(table, ids, scale=1.0, dtype=None):
@@ -161,7 +164,7 @@ def lookup(table, ids, scale=1.0, dtype=None):
 
   table: [rows, dims], float32, float16 or bfloat16, rows contiguous; ids: int32 or int64 of any shape; the result, of
   shape [*ids.shape, dims], has the table's type or is float32.  Products are taken in 32 bits and rounded once.
-  Differentiable with respect to table (once): see lookup_grad.  Where a backward pass is captured into a graph, no eager
+  Differentiable with respect to table (once, and in reverse: a table with a forward-mode tangent is refused): see lookup_grad.  Where a backward pass is captured into a graph, no eager
   graph over the same table may be alive (its leaf belongs to another stream then, which torch would wait for)."""
   _tensor(table, "table", 2)
   _tensor(ids, "ids", types=_IDS)
@@ -169,12 +172,13 @@ def lookup(table, ids, scale=1.0, dtype=None):
   dtype = dtype or table.dtype
   _check(dtype is table.dtype or dtype is torch.float32, "the result has the table's type or is float32")
   _check(table.shape[1] > 0, "the table's rows are empty")
-  _rows(table, "table")
+  stride = _rows(table, "table")
+  _check(_tangent(table).tangent is None, "lookup has no forward-mode derivative")
   device = _same_device(table, ids)
   flat, shape = _flat(ids), None if ids.dim() == 1 else (*ids.shape, table.shape[1])
   if table.requires_grad and torch.is_grad_enabled():
-    return _Lookup.apply(table, flat, shape, scale, dtype, device)
-  out = _lookup(table, flat, scale, dtype, device)
+    return _Lookup.apply(table, stride, flat, shape, scale, dtype, device)
+  out = _lookup(table, stride, flat, scale, dtype, device)
   return out if shape is None else out.view(shape)
 
 

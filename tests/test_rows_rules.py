@@ -28,3 +28,20 @@ def test_products_of_bad_sizes_have_no_plan():
   for sizes in ((0, 8, 32, 0, 1), (5, 0, 32, 0, 1), (5, 8, 0, 0, 1), (5, 8, 32, 3, 1), (5, 8, 32, 0, 0)):
     assert capi.load().cuhnsw_packed_scores_plan(*sizes, out) == -1
   assert capi.load().cuhnsw_packed_scores_plan(5, 8, 32, 0, 1, None) == -1
+
+
+def test_a_lookup_drops_no_tangent():
+  """A table of forward-mode differentiation does not require a gradient: its tangent would be lost without a word."""
+  torch = pytest.importorskip("torch")
+  from torch.autograd import forward_ad
+
+  from cuhnsw_amd import rows
+  ids = torch.zeros(1, dtype=torch.int64)
+  with forward_ad.dual_level():
+    for table in (torch.zeros(4, 3), torch.zeros(4, 3, requires_grad=True)):
+      with pytest.raises(ValueError, match="forward-mode"):
+        rows.lookup(forward_ad.make_dual(table, torch.ones(4, 3)), ids)
+    with pytest.raises(ValueError, match="on the GPU"):    # (one without a tangent is not refused for it)
+      rows.lookup(torch.zeros(4, 3), ids)
+  with pytest.raises(ValueError, match="forward-mode"):
+    torch.func.jvp(lambda x: rows.lookup(x, ids), (torch.zeros(4, 3),), (torch.ones(4, 3),))
