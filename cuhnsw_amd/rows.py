@@ -60,6 +60,7 @@ def _tensor(x, name, dims=None, types=_TYPES):
     raise TypeError("%s is a tensor, not %s" % (name, type(x).__name__))
   _check(dims is None or x.dim() == dims, "%s has %s dimensions, %s are wanted", name, x.dim(), dims)
   _check(x.dtype in types, "%s has the type %s: %s is wanted", name, x.dtype, " or ".join(str(t) for t in types))
+  _check(not x.is_neg(), "%s is a view that is still to be negated (resolve_neg)", name)
 
 
 def _rows(x, name):
@@ -422,6 +423,7 @@ def reorder_states(states, parents):
   for x in states:
     if not isinstance(x, torch.Tensor):
       raise TypeError("states is a list of tensors")
+    _check(not (x.is_neg() or x.is_conj()), "a state is a view that is still to be negated or conjugated (resolve_neg, resolve_conj)")
     shape, stride, size = x.shape, x.stride(), x.element_size()
     _check(len(shape) >= 2 and shape[0] == b and shape[1] == k and k > 0, "states have the shape [batch, beams, ...]: %s with %d batch entries",
            tuple(shape), b)

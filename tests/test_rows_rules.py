@@ -45,3 +45,25 @@ def test_a_lookup_drops_no_tangent():
       rows.lookup(torch.zeros(4, 3), ids)
   with pytest.raises(ValueError, match="forward-mode"):
     torch.func.jvp(lambda x: rows.lookup(x, ids), (torch.zeros(4, 3),), (torch.ones(4, 3),))
+
+
+def test_views_that_are_still_to_be_negated_or_conjugated_are_refused():
+  """What is in their memory is not what they stand for."""
+  torch = pytest.importorskip("torch")
+  from cuhnsw_amd import rows
+  late = torch.zeros(2, 4, 64, dtype=torch.complex64).conj()
+  negated = late.imag
+  assert negated.is_neg() and late.is_conj()
+  ids, parents = torch.zeros(2, dtype=torch.int64), torch.zeros(2, 4, dtype=torch.int32)
+  flat = torch.zeros(4, dtype=torch.complex64).conj().imag
+  for call in (lambda: rows.lookup(negated[0], ids), lambda: rows.lookup_grad(negated[0, :2], ids, 3), lambda: rows.pack(negated[0]),
+               lambda: rows.select_beams(negated, None, 1), lambda: rows.select_beams(torch.zeros(2, 4, 64), negated[:, :, 0], 1),
+               lambda: rows.reorder_states([negated], parents), lambda: rows.reorder_states([late], parents)):
+    with pytest.raises(ValueError, match="still to be negated"):
+      call()
+  assert flat.is_neg()
+  packed = object.__new__(rows.PackedRows)
+  packed.num_rows, packed.num_dims = 4, 64
+  for call in (lambda: packed.scores(negated[0]), lambda: packed.scores(torch.zeros(1, 64), bias=flat), lambda: packed.search_knn(negated[0], 1)):
+    with pytest.raises(ValueError, match="still to be negated"):
+      call()
