@@ -427,9 +427,9 @@ def reorder_states(states, parents):
     shape, stride, size = x.shape, x.stride(), x.element_size()
     _check(len(shape) >= 2 and shape[0] == b and shape[1] == k and k > 0, "states have the shape [batch, beams, ...]: %s with %d batch entries",
            tuple(shape), b)
-    expected = 1
+    expected, empty = 1, x.numel() == 0
     for i in range(len(shape) - 1, 1, -1):
-      _check(shape[i] == 1 or stride[i] == expected, "one beam's state has to be contiguous")
+      _check(empty or shape[i] == 1 or stride[i] == expected, "one beam's state has to be contiguous")
       expected *= shape[i]
     sizes.append(expected * size)
     strides_b.append(stride[0] * size)

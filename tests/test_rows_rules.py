@@ -67,3 +67,11 @@ def test_views_that_are_still_to_be_negated_or_conjugated_are_refused():
   for call in (lambda: packed.scores(negated[0]), lambda: packed.scores(torch.zeros(1, 64), bias=flat), lambda: packed.search_knn(negated[0], 1)):
     with pytest.raises(ValueError, match="still to be negated"):
       call()
+
+
+def test_states_without_elements_are_contiguous():
+  torch = pytest.importorskip("torch")
+  from cuhnsw_amd import rows
+  for shape in ((2, 3, 2, 0, 3), (2, 3, 0), (2, 3, 5, 0)):
+    with pytest.raises(ValueError, match="on the GPU"):
+      rows.reorder_states([torch.zeros(shape)], torch.zeros(2, 3, dtype=torch.int32))
