@@ -301,7 +301,7 @@ class PackedRows:
     l2 = dist_type == "l2"
     bias = -self.norms() if l2 else None
     lengths = q.double().square().sum(1, keepdim=True) if l2 else None
-    step = max(1, (1 << 30) // max(1, self.num_rows))  # (scores of at most 4 GiB at a time)
+    step = max(1, min(1 << 22, (1 << 30) // self.num_rows))  # (scores of at most 4 GiB at a time, and queries that one product takes)
     found = []
     for low in range(0, max(1, q.shape[0]), step):
       part = self.scores(q[low:low + step], alpha=2.0 if l2 else 1.0, bias=bias, dtype=torch.float32)
