@@ -478,7 +478,7 @@ struct GradScratch {
     }
     counts = s.part<int>((size_t)p.blocks << p.bits);
     long_sums = s.part<float>((size_t)(num_ids / kLong) * num_dims);
-    bounds = s.part<int>((size_t)num_rows + 2);  // (at least a row for every workgroup)
+    bounds = s.part<int>((size_t)num_rows / 4 + 2);  // (every workgroup but the last has four rows or more: one for each group of lanes)
     bytes = s.used();
   }
 };

@@ -75,3 +75,10 @@ def test_states_without_elements_are_contiguous():
   for shape in ((2, 3, 2, 0, 3), (2, 3, 0), (2, 3, 5, 0)):
     with pytest.raises(ValueError, match="on the GPU"):
       rows.reorder_states([torch.zeros(shape)], torch.zeros(2, 3, dtype=torch.int32))
+
+
+def test_scratch_memory_of_a_gradient_does_not_grow_with_the_rows_more_than_it_has_to():
+  """Sorted ids, sums of long stretches, counts: by the ids.  By the rows: where those of every workgroup begin, four rows or more."""
+  l = capi.load()
+  few, many = (l.cuhnsw_lookup_grad_workspace(5000, n, 8) for n in (1 << 20, 1 << 30))
+  assert 0 < many - few <= (1 << 30) + (1 << 20)     # (the counts have more digits)
