@@ -1,7 +1,7 @@
 // Rows of a table by id, and the gradient of that.
 //
 //   out[t] = scale * table[ids[t]]                         (zeros where ids[t] is outside [0, num_rows))
-//   grad[v] = scale * sum over t with ids[t] = v of g[t]   (t ascending; zeros for rows that no id names)
+//   grad[v] = scale * sum over t with ids[t] = v of g[t]   (zeros for rows that no id names; in which order is fixed by sizes and ids)
 //
 // Products and sums are held in 32 bits and rounded once, to nearest, when they are stored.
 #include <algorithm>
@@ -60,8 +60,8 @@ void with_vector(int num_dims, F&& f) {
 
 // ---------------------------------------------------------------------------------------------- lookup
 // Bound by memory: each row is fetched once and written once, four rows of a lane's in flight (from 2048 workgroups on, below that there
-// are too few rows for four each).  50 003 of 400 000 rows of 960 float16: 192 MB in 38.5 us, 5.0 TB/s, what a copy reaches; 65 536
-// tokens of 1024 bfloat16 46 us.  A few rows take a launch: 3 us.
+// are too few rows for four each).  50 003 of 400 000 rows of 960 float16: 192 MB in 37.5 us, 5.1 TB/s (a copy of as much takes 39 us,
+// 5.2 TB/s); 65 536 tokens of 1024 bfloat16 46 us.  A few rows take a launch: 3 us.
 template <typename T, typename U, int VE, bool STREAMED>
 __global__ void __launch_bounds__(256) lookup_kernel(const T* table, long long num_rows, long long row_stride, int num_dims,
                                                      const void* ids, int ids_64, long long num_ids, float scale, U* out, int lanes) {

@@ -89,7 +89,9 @@ void launch_pack(const PackArgs& a, hipStream_t stream) {
 //
 // Queries are laid out as the lanes want them: for a tile of 16 queries and a unit of 32 elements, 16 bytes for every quarter of the
 // unit and query.  That is a launch of its own (prepare_kernel), or, of one or two, every workgroup's first step, into its LDS.
-constexpr int kManyWaves = 4, kManyResident = 768;  // wavefronts of a workgroup for many queries, and such workgroups that the machine holds
+constexpr int kManyWaves = 4;      // wavefronts of a workgroup for many queries
+constexpr int kManyResident = 768;  // such workgroups at work at a time, as the plan counts: three on a CU (the instances' registers and LDS
+                                    // let it hold two to six: two with float32 queries, four tiles and chunks of four units)
 constexpr int kTile = 16, kUnit = 32, kRowTiles = 4;  // queries or rows of a matrix product, elements of it; row tiles of a wavefront
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -199,7 +201,8 @@ __global__ void __launch_bounds__(256) prepare_kernel(ScoresArgs a, int planes) 
 }
 
 // The eight codes of a word, less 8 or as they are, as float16, in the order 0 4 1 5 2 6 3 7: a code behind the exponent of 1024
-// is 1024 more (16 times the code behind it for every other one), and what is too much goes off exactly.
+// is 1024 more (16 times the code behind it for every other one), and what is too much goes off exactly (the well-known way to
+// small whole numbers in floating point, by the exponent below which their bits lie).
 template <bool CENTRED>
 __device__ inline half8_t codes_of(uint32_t word) {
   constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;

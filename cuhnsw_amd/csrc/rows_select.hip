@@ -5,9 +5,12 @@
 //   the `num` largest totals of b over (k, v), largest first; of equal ones the lower k first, then the larger x, then the
 //   lower v.
 //
-// Totals are held in 64 bits: candidates of different beams meet there, and a rounding must not order them.  A NaN counts as
-// -infinity, and what is -infinity is never chosen: places that are left over say -infinity, parent -1, token -1.  A finished
-// beam has one candidate, the token `end` with the beam's own score.
+// Totals are formed, held and compared in 64 bits; the sum in them is one of the machine's exponentials in float32, joined in 64
+// bits, and good to about 2^-20 of itself: candidates of different beams whose totals are nearer than that may stand in either
+// order, those of one beam stand in the scores' own.  A NaN counts as -infinity, and what is -infinity is never chosen: places that are
+// left over say -infinity, parent -1, token -1.  Where a score is +infinity the formula has no value, and only the beam's n
+// infinite ones are candidates, each with total beams[b][k] - log(n).  A finished beam has one candidate, the token `end` with
+// the beam's own score.
 #include <algorithm>
 
 #include "../../include/cuhnsw_amd.h"
@@ -134,7 +137,7 @@ __device__ inline int keep_best(uint64_t* keys, int count, int most, int (&count
 // overflow meanwhile (scores in an order that is hard) those tiles are gone over again, a score of each thread at a time.
 //
 // What a score costs: its conversion, a comparison, and normalised the maximum, a subtraction, a product, the exponential (of four
-// times the cost) and an addition.  100 rows of 1 183 514 float32, the best 100: 105 us, 4.5 TB/s, what a copy reaches;
+// times the cost) and an addition.  100 rows of 1 183 514 float32, the best 100: 103 us, 4.6 TB/s of reads;
 // 32 x 8 rows of 131 072 bfloat16, normalised: 34 us, 2.0 TB/s, bound by these instructions.
 //
 // (Tiles of 4 float32 for each thread instead of 16 are up to 0.5 us faster where rows are few and short, 5 of 28 slower at 128

@@ -9,8 +9,8 @@
 
 Every call runs on its tensors' device and torch's current stream there, does not wait for the GPU, takes its scratch
 memory from torch, and may be captured into a graph (pack_index waits, and may not; PackedRows.norms waits once).  lookup
-is differentiable, the others are not: their results carry no gradient and no tangent.  Wrong arguments are a ValueError (a TypeError where the kind of
-object is wrong); what the native library refuses is a RuntimeError with its message, as everywhere in this package.
+is differentiable, the others are not: their results carry no gradient and no tangent, whatever their inputs do.  Wrong
+arguments are a ValueError (a TypeError where the kind of object is wrong); what the native library refuses is a RuntimeError with its message, as everywhere in this package.
 There is no CPU form.
 
 torch ships its own copy of the HIP runtime: it has to be imported before this package's native library is loaded, or
@@ -165,8 +165,9 @@ def lookup(table, ids, scale=1.0, dtype=None):
 
   table: [rows, dims], float32, float16 or bfloat16, rows contiguous; ids: int32 or int64 of any shape; the result, of
   shape [*ids.shape, dims], has the table's type or is float32.  Products are taken in 32 bits and rounded once.
-  Differentiable with respect to table (once, and in reverse: a table with a forward-mode tangent is refused): see lookup_grad.  Where a backward pass is captured into a graph, no eager
-  graph over the same table may be alive (its leaf belongs to another stream then, which torch would wait for)."""
+  Differentiable with respect to table (once, and in reverse: a table with a forward-mode tangent is refused): see
+  lookup_grad.  Where a backward pass is captured into a graph, no eager graph over the same table may be alive (its leaf
+  belongs to another stream then, which torch would wait for)."""
   _tensor(table, "table", 2)
   _tensor(ids, "ids", types=_IDS)
   scale = _number(scale, "scale")
@@ -187,7 +188,8 @@ def lookup_grad(grad, ids, num_rows, scale=1.0, dtype=None):
   """The gradient of lookup with respect to its table: [num_rows, dims], row v the sum of scale * grad[t] over the places
   t with ids[t] = v.
 
-  grad: [*ids.shape, dims].  The sums are formed in 32 bits, in an order that depends on the ids alone, and rounded once to
+  grad: [*ids.shape, dims]; at most 2^30 ids and 2^31 - 2 rows.  The sums are formed in 32 bits, in an order that depends on the sizes and the
+  ids alone, and rounded once to
   `dtype` (grad's own, or any where grad is float32): the same inputs give the same bits."""
   _tensor(grad, "grad")
   _tensor(ids, "ids", types=_IDS)
@@ -241,8 +243,9 @@ class PackedRows:
   def scores(self, queries, alpha=1.0, bias=None, dtype=None):
     """alpha * queries @ rows.T (+ bias): [num_queries, num_rows], of the queries' type or float32.
 
-    queries: [num_queries, num_dims] (or one: [num_dims]), float32, float16 or bfloat16; bias: float32 [num_rows].  Sums are
-    held in 32 bits.  A query that is not finite gets scores that are not."""
+    queries: [num_queries, num_dims] (or one: [num_dims]), at most 16 777 200, float32, float16 or bfloat16; bias: float32
+    [num_rows].  Sums are held in 32 bits; a float32 query as two planes of float16, good to 2^-23 of an element or 2^-39 of its largest
+    one.  A query that is not finite gets scores that are not."""
     _tensor(queries, "queries")
     _check(queries.dim() in (1, 2) and queries.shape[-1] == self.num_dims, "queries have the shape [num_queries, %d]", self.num_dims)
     alpha = _number(alpha, "alpha")
@@ -288,7 +291,8 @@ class PackedRows:
 
   def search_knn(self, queries, topk, dist_type="dot"):
     """The topk (up to 256) nearest of all rows: (ids int32, or int64 labels, distances float32, found int32), nearest first and of
-    equal ones the lower row first, as CuHNSW.search_knn's: -<q, row> for "dot", squared distances for "l2"."""
+    equal ones the lower row first, as CuHNSW.search_knn's: -<q, row> for "dot", squared distances for "l2" (|q|^2 + |row|^2 - 2 <q, row>, of
+    which the last two are formed in 32 bits: a distance that is small beside the lengths is as exact as these)."""
     _check(dist_type in ("dot", "l2"), "dist_type is dot or l2, not %s", dist_type)
     _tensor(queries, "queries")
     q = queries if queries.dim() == 2 else queries[None]
@@ -371,11 +375,14 @@ def select_beams(scores, beams, num, normalise=True, finished=None, end=None):
   scores: [batch, beams, values], float32, float16 or bfloat16; beams: float32 [batch, beams], what the beams have gathered, or
   None (zeros).  A candidate's total is beams + scores, with normalise beams + log_softmax(scores); totals are compared in 64
   bits, equal ones go to the lower beam, then the larger score, then the lower token.  Masked places hold -infinity (a NaN counts as
-  one): they are never chosen, and where too few candidates are left the rest says -infinity, -1, -1.  finished: bool
-  [batch, beams] or None: a finished beam has one candidate, token `end`, with what it gathered.
+  one): they are never chosen, and where too few candidates are left the rest says -infinity, -1, -1.  With normalise, where a
+  score is +infinity (and log_softmax is a NaN) only the beam's n infinite ones are candidates, each with total beams - log(n).
+  finished: bool [batch, beams] or None: a finished beam has one candidate, token `end`, with what it gathered.
 
-  The same call gives the same answer to the last bit; how a row's sum of exponentials is split depends on the sizes, so that
-  a row's totals can differ in their last bits between batches of different sizes."""
+  A beam's own candidates stand in the order of their scores; log_softmax is good to about 2^-20, and candidates of different
+  beams that are nearer to each other may stand in either order.  The same call gives the same answer to the last bit; how a
+  row's sum of exponentials is split depends on the sizes, so that a row's totals can differ in their last bits between batches
+  of different sizes."""
   _tensor(scores, "scores", 3)
   _check(isinstance(num, int) and 0 < num <= 256, "num is between 1 and 256")
   b, k, v = scores.shape

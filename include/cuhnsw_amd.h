@@ -319,7 +319,7 @@ int cuhnsw_lookup_rows_grad(const void* grad, int grad_type, long long grad_stri
  *
  * cuhnsw_pack_rows: the nearest such rows of finite ones (scale = largest magnitude / 7, or the span / 15 with offsets).
  * cuhnsw_packed_scores: out[m][n] = alpha * <row n, query m> + bias[n] (bias: float32 [num_rows] or NULL), of the queries'
- *   type or float32.  A query that holds an infinity or a NaN gets NaN or infinities; other queries are not touched by it.
+ *   type or float32.  At most 16 777 200 queries and 2^31 - 1024 rows.  A query that holds an infinity or a NaN gets NaN or infinities; other queries are not touched by it.
  * cuhnsw_packed_scores_plan: how such a call goes, in four numbers: [0] tiles of 16 queries that a wavefront of the kernel for
  *   many queries has at a time, 0 where the call goes to the kernel for few; [1] blocks of these tiles that its workgroup goes
  *   over; [2] wavefronts of the kernel for few that share a row; [3] whether its workgroups lay the queries out themselves.
@@ -339,7 +339,9 @@ int cuhnsw_packed_scores(const void* codes, const void* scales, const void* offs
  *     beams[b][k] + scores[b][k][v] - log(sum over u of exp(scores[b][k][u]))
  *   over k and v, largest first; of equal totals (held in 64 bits) the lower k first, then the larger score, then the lower
  *   v.  beams: float32 [num_batch, num_beams] or NULL (zeros).  A NaN counts as -infinity and -infinity is never chosen: places
- *   that are left over say -infinity, -1, -1.  finished (bytes, [num_batch, num_beams]) or NULL: where it is not 0 the beam
+ *   that are left over say -infinity, -1, -1.  With normalise, where a score is +infinity only the beam's n infinite ones are
+ *   candidates, each with total beams[b][k] - log(n).  The sum is good to about 2^-20 of itself: candidates of different beams that are
+ *   nearer to each other may stand in either order.  finished (bytes, [num_batch, num_beams]) or NULL: where it is not 0 the beam
  *   has one candidate, token `end` with total beams[b][k].  num_values <= 2^30, num_beams <= 1024, num_beams * min(num, num_values) <= 4096.  Results: dense
  *   [num_batch, num].  (One beam, not normalised: the num nearest neighbours of a matrix of scores.)
  * cuhnsw_reorder_states: for each of num_states arrays to[b][j] = from[b][parents[b][j]], zeros where the parent is outside
